@@ -54,6 +54,8 @@
 #include "dft2stage.h"
 #include "gru_clusterx.h"
 #include "dft64.h"
+#include "gated_delta.h"
+#include "w4_matvec.h"
 
 // ------------------------------------------------------------------------------------------------
 // HIP multiplexes every stream of the process onto GPU_MAX_HW_QUEUES hardware queues (default 4); the engine runs four
@@ -171,6 +173,7 @@ extern "C" size_t dpdf_manifest_text(const dpdf_cfg* cfg, char* buf, size_t cap)
 #include "host_batch_calls.h"
 #include "host_streaming.h"
 #include "host_stream_pool.h"
+#include "host_operators.h"
 extern "C" int dpdf_streams_process(dpdf_streams* s, const float* pcm_in, int n_hops, float* pcm_out, int flags) {
     return dpdf_streams_process_masked(s, pcm_in, n_hops, pcm_out, nullptr, flags);
 }

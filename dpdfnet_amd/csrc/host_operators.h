@@ -1,0 +1,190 @@
+// host_operators.h -- C entry points of the stand-alone operators (gated_delta.h, w4_matvec.h): device pointers, the caller's stream, nothing
+// allocated, nothing waited for, so that every call can be captured into a graph.  Arguments are checked before anything is launched.
+
+namespace {
+struct OpDevice {                                 // the call's device for as long as it runs, the caller's afterwards
+    int before = -1; hipError_t err;
+    explicit OpDevice(int device) {
+        err = hipGetDevice(&before);
+        if (err == hipSuccess && before != device) err = hipSetDevice(device);
+        else before = -1;
+    }
+    ~OpDevice() { if (before >= 0) (void)hipSetDevice(before); }
+};
+
+struct OpSpan { const char* lo; const char* hi; };
+OpSpan op_span(const void* p, const long* stride, const long* size, int dims, long last, int elem) {
+    long n = last;
+    for (int i = 0; i < dims; ++i) n += (size[i] - 1) * stride[i];
+    return {(const char*)p, (const char*)p + n * elem};
+}
+bool op_meet(const OpSpan& x, const OpSpan& y) { return x.lo < y.hi && y.lo < x.hi; }
+// no two elements of an output in one place: every dimension steps over all that the smaller steps span
+bool op_apart(const long* stride, const long* size, int dims, long last) {
+    bool used[3] = {false, false, false};
+    long span = last;
+    for (int k = 0; k < dims; ++k) {
+        int best = -1;
+        for (int i = 0; i < dims; ++i) if (!used[i] && (best < 0 || stride[i] < stride[best] || (stride[i] == stride[best] && size[i] < size[best]))) best = i;
+        used[best] = true;
+        if (size[best] == 1) continue;
+        if (stride[best] < span) return false;
+        span += (size[best] - 1) * stride[best];
+    }
+    return true;
+}
+int op_bytes(int dtype) { return dtype == DPDF_F32 ? 4 : dtype == DPDF_F16 || dtype == DPDF_BF16 ? 2 : 0; }
+bool op_aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+
+int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
+    if (!p) return set_err(DPDF_E_INVALID, "null argument");
+    const dpdf_gated_delta_args& x = *p;
+    const int e = op_bytes(x.dtype), ge = op_bytes(x.gate_dtype);
+    if (!e || !ge || (x.gate_dtype != DPDF_F32 && x.gate_dtype != x.dtype)) return set_err(DPDF_E_INVALID, "gated delta rule: unsupported dtypes %d / %d", x.dtype, x.gate_dtype);
+    if (x.batch < 0 || x.frames < 0) return set_err(DPDF_E_INVALID, "gated delta rule: negative size batch=%d frames=%d", x.batch, x.frames);
+    if (x.k_heads < 1 || x.v_heads < 1 || x.v_heads % x.k_heads) return set_err(DPDF_E_INVALID, "gated delta rule: %d value heads are no multiple of %d key heads", x.v_heads, x.k_heads);
+    if (x.k_dim < 1 || x.k_dim > 128 || x.v_dim < 1) return set_err(DPDF_E_INVALID, "gated delta rule: head sizes %d (1 .. 128) and %d (from 1)", x.k_dim, x.v_dim);
+    if (!(x.scale - x.scale == 0.f)) return set_err(DPDF_E_INVALID, "gated delta rule: scale is not finite");
+    if (step && x.lengths) return set_err(DPDF_E_INVALID, "gated delta rule: a step takes no lengths");
+    if (!step && x.active) return set_err(DPDF_E_INVALID, "gated delta rule: clips take no mask of active streams");
+    const long B = x.batch, T = x.frames, Hk = x.k_heads, Hv = x.v_heads, Dk = x.k_dim, Dv = x.v_dim;
+    const long states = (Dv + 31) / 32 * B * Hv;
+    if (states > 0x7fffffffL) return set_err(DPDF_E_INVALID, "gated delta rule: batch %d with %d heads of %d is too large for one call", x.batch, x.v_heads, x.v_dim);
+    if (B && (step && (!x.state_in || !x.state_out))) return set_err(DPDF_E_INVALID, "gated delta rule: a step needs its state");
+    const long kd[3] = {B, T, Hk}, vd[3] = {B, T, Hv};
+    for (const long* s : {x.q_stride, x.k_stride, x.v_stride, x.g_stride, x.beta_stride, x.out_stride})
+        for (int i = 0; i < 3; ++i) if (s[i] < 0) return set_err(DPDF_E_INVALID, "gated delta rule: negative stride");
+    const long n = B * Hv * Dk * Dv * 4;
+    const OpSpan si = {(const char*)x.state_in, (const char*)x.state_in + (x.state_in ? n : 0)}, so = {(const char*)x.state_out, (const char*)x.state_out + (x.state_out ? n : 0)};
+    if (B && T) {
+        if (!x.q || !x.k || !x.v || !x.g || !x.beta || !x.out) return set_err(DPDF_E_INVALID, "null argument");
+        if (!op_aligned(x.q, e) || !op_aligned(x.k, e) || !op_aligned(x.v, e) || !op_aligned(x.out, e) || !op_aligned(x.g, ge) || !op_aligned(x.beta, ge))
+            return set_err(DPDF_E_INVALID, "gated delta rule: a pointer is not aligned to its type");
+        if (!op_apart(x.out_stride, vd, 3, Dv)) return set_err(DPDF_E_INVALID, "gated delta rule: elements of out share memory");
+        const OpSpan o = op_span(x.out, x.out_stride, vd, 3, Dv, e);
+        const OpSpan in[5] = {op_span(x.q, x.q_stride, kd, 3, Dk, e), op_span(x.k, x.k_stride, kd, 3, Dk, e), op_span(x.v, x.v_stride, vd, 3, Dv, e),
+                              op_span(x.g, x.g_stride, vd, 3, 1, ge), op_span(x.beta, x.beta_stride, vd, 3, 1, ge)};
+        for (const OpSpan& i : in) if (op_meet(o, i) || op_meet(so, i)) return set_err(DPDF_E_INVALID, "gated delta rule: an output overlaps an input");
+        if (op_meet(o, si) || op_meet(o, so)) return set_err(DPDF_E_INVALID, "gated delta rule: out overlaps a state");
+    }
+    if (x.state_in != x.state_out && op_meet(si, so)) return set_err(DPDF_E_INVALID, "gated delta rule: the states overlap in part");
+    if (!op_aligned(x.state_in, 4) || !op_aligned(x.state_out, 4) || !op_aligned(x.lengths, 4)) return set_err(DPDF_E_INVALID, "gated delta rule: a pointer is not aligned to its type");
+    a.q = x.q; a.k = x.k; a.v = x.v; a.g = x.g; a.beta = x.beta; a.out = x.out;
+    a.state_in = x.state_in; a.state_out = x.state_out; a.lengths = x.lengths; a.active = x.active;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = x.q_stride[i]; a.ks[i] = x.k_stride[i]; a.vs[i] = x.v_stride[i];
+        a.gs[i] = x.g_stride[i]; a.bs[i] = x.beta_stride[i]; a.os[i] = x.out_stride[i];
+    }
+    a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale;
+    return DPDF_OK;
+}
+
+template <typename T, typename G>
+void gd_launch_step(const GatedDeltaArgs& a, unsigned grid, bool vec, hipStream_t s) {
+#define GD_STEP(D) (vec ? (gated_delta_step_kernel<T, G, D, true><<<grid, 64, 0, s>>>(a)) : (gated_delta_step_kernel<T, G, D, false><<<grid, 64, 0, s>>>(a)))
+    if (a.Dk <= 16) GD_STEP(16); else if (a.Dk <= 32) GD_STEP(32); else if (a.Dk <= 64) GD_STEP(64); else GD_STEP(128);
+#undef GD_STEP
+}
+template <typename T, typename G>
+void gd_launch_clip(const GatedDeltaArgs& a, unsigned grid, hipStream_t s) {
+    if (a.Dk <= 16) gated_delta_clip_kernel<T, G, 16><<<grid, 256, 0, s>>>(a);
+    else if (a.Dk <= 32) gated_delta_clip_kernel<T, G, 32><<<grid, 256, 0, s>>>(a);
+    else if (a.Dk <= 64) gated_delta_clip_kernel<T, G, 64><<<grid, 256, 0, s>>>(a);
+    else gated_delta_clip_kernel<T, G, 128><<<grid, 256, 0, s>>>(a);
+}
+// calls f with the types of the values and of the gates
+template <typename F> void gd_types(int dtype, int gate, F f) {
+    if (dtype == DPDF_F32) f(float(), float());
+    else if (dtype == DPDF_F16) { if (gate == DPDF_F32) f(__half(), float()); else f(__half(), __half()); }
+    else { if (gate == DPDF_F32) f(__hip_bfloat16(), float()); else f(__hip_bfloat16(), __hip_bfloat16()); }
+}
+
+int w4_check(int dtype, long K, long N, int group, const char* what) {
+    if (!op_bytes(dtype)) return set_err(DPDF_E_INVALID, "%s: unsupported dtype %d", what, dtype);
+    if (K < 1 || N < 1) return set_err(DPDF_E_INVALID, "%s: empty layer %ld x %ld", what, N, K);
+    if (group < 32 || group % 32) return set_err(DPDF_E_INVALID, "%s: group %d is no multiple of 32", what, group);
+    return DPDF_OK;
+}
+}  // namespace
+
+extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* stream) {
+    GatedDeltaArgs a;
+    if (int rc = gd_check(args, false, a)) return rc;
+    if (!args->batch || (!args->frames && !args->state_out)) return DPDF_OK;
+    OpDevice dev(device);
+    HIP_TRY(dev.err);
+    a.strips = (a.Dv + 63) / 64;
+    const unsigned grid = (unsigned)((long)args->batch * a.Hv * a.strips);
+    gd_types(args->dtype, args->gate_dtype, [&](auto t, auto g) { gd_launch_clip<decltype(t), decltype(g)>(a, grid, (hipStream_t)stream); });
+    HIP_TRY(hipGetLastError());
+    return DPDF_OK;
+}
+
+extern "C" int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* args, void* stream) {
+    GatedDeltaArgs a;
+    if (int rc = gd_check(args, true, a)) return rc;
+    if (!args->batch || !args->frames) return DPDF_OK;
+    OpDevice dev(device);
+    HIP_TRY(dev.err);
+    a.strips = (a.Dv + 31) / 32;
+    const unsigned grid = (unsigned)((long)args->batch * a.Hv * a.strips);
+    const bool vec = a.Dv % 4 == 0 && op_aligned(a.state_in, 16) && op_aligned(a.state_out, 16);
+    gd_types(args->dtype, args->gate_dtype, [&](auto t, auto g) { gd_launch_step<decltype(t), decltype(g)>(a, grid, vec, (hipStream_t)stream); });
+    HIP_TRY(hipGetLastError());
+    return DPDF_OK;
+}
+
+extern "C" int dpdf_w4_quantize(int device, const dpdf_w4_quantize_args* args, void* stream) {
+    if (!args) return set_err(DPDF_E_INVALID, "null argument");
+    const dpdf_w4_quantize_args& x = *args;
+    if (int rc = w4_check(x.dtype, x.in_dim, x.out_dim, x.group, "w4 quantize")) return rc;
+    const long groups = ((long)x.in_dim + x.group - 1) / x.group, bytes = ((long)x.in_dim + 1) / 2;
+    if (!x.weight || !x.codes || !x.scales) return set_err(DPDF_E_INVALID, "null argument");
+    if (x.weight_stride < 0 || x.codes_pitch < bytes || x.scales_stride < groups || (x.zeros && x.zeros_pitch < groups))
+        return set_err(DPDF_E_INVALID, "w4 quantize: rows overlap");
+    const int e = op_bytes(x.dtype);
+    if (!op_aligned(x.weight, e) || !op_aligned(x.scales, e)) return set_err(DPDF_E_INVALID, "w4 quantize: a pointer is not aligned to its type");
+    const long rows = x.out_dim, n[1] = {rows};
+    const OpSpan w = op_span(x.weight, &x.weight_stride, n, 1, x.in_dim, e), o[3] = {op_span(x.codes, &x.codes_pitch, n, 1, bytes, 1), op_span(x.scales, &x.scales_stride, n, 1, groups, e),
+                     {(const char*)x.zeros, (const char*)x.zeros + (x.zeros ? (rows - 1) * x.zeros_pitch + groups : 0)}};
+    for (int i = 0; i < 3; ++i)
+        if (op_meet(w, o[i]) || op_meet(o[i], o[(i + 1) % 3])) return set_err(DPDF_E_INVALID, "w4 quantize: an output overlaps another tensor");
+    if ((long)x.out_dim * groups > 4 * 0x7fffffffL) return set_err(DPDF_E_INVALID, "w4 quantize: %d x %ld groups are too many for one call", x.out_dim, groups);
+    OpDevice dev(device);
+    HIP_TRY(dev.err);
+    W4QuantArgs a{x.weight, x.weight_stride, x.codes, x.codes_pitch, x.scales, x.scales_stride, x.zeros, x.zeros_pitch, x.out_dim, x.in_dim, x.group, (int)groups};
+    const unsigned grid = (unsigned)(((long)x.out_dim * groups + 3) / 4);
+    if (x.dtype == DPDF_F32) w4_quantize_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    else if (x.dtype == DPDF_F16) w4_quantize_kernel<__half><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    else w4_quantize_kernel<__hip_bfloat16><<<grid, 256, 0, (hipStream_t)stream>>>(a);
+    HIP_TRY(hipGetLastError());
+    return DPDF_OK;
+}
+
+extern "C" int dpdf_w4_matvec(int device, const dpdf_w4_matvec_args* args, void* stream) {
+    if (!args) return set_err(DPDF_E_INVALID, "null argument");
+    const dpdf_w4_matvec_args& x = *args;
+    if (int rc = w4_check(x.dtype, x.in_dim, x.out_dim, x.group, "w4 matvec")) return rc;
+    if (x.scale_dtype != DPDF_F32 && x.scale_dtype != x.dtype) return set_err(DPDF_E_INVALID, "w4 matvec: unsupported dtypes %d / %d", x.dtype, x.scale_dtype);
+    if (x.rows < 0) return set_err(DPDF_E_INVALID, "w4 matvec: negative size rows=%d", x.rows);
+    if (!x.rows) return DPDF_OK;
+    const long groups = ((long)x.in_dim + x.group - 1) / x.group, bytes = ((long)x.in_dim + 1) / 2;
+    if (!x.x || !x.codes || !x.scales || !x.out) return set_err(DPDF_E_INVALID, "null argument");
+    if (x.x_stride < 0 || x.codes_pitch < 0 || x.scales_stride < 0 || x.zeros_pitch < 0) return set_err(DPDF_E_INVALID, "w4 matvec: negative stride");
+    if (x.rows > 1 && x.out_stride < x.out_dim) return set_err(DPDF_E_INVALID, "w4 matvec: elements of out share memory");
+    const int e = op_bytes(x.dtype), se = op_bytes(x.scale_dtype);
+    if (!op_aligned(x.x, e) || !op_aligned(x.out, e) || !op_aligned(x.bias, e) || !op_aligned(x.scales, se)) return set_err(DPDF_E_INVALID, "w4 matvec: a pointer is not aligned to its type");
+    const long rows[1] = {x.rows}, outs[1] = {x.out_dim};
+    const OpSpan o = op_span(x.out, &x.out_stride, rows, 1, x.out_dim, e);
+    const OpSpan in[5] = {op_span(x.x, &x.x_stride, rows, 1, x.in_dim, e), op_span(x.codes, &x.codes_pitch, outs, 1, bytes, 1), op_span(x.scales, &x.scales_stride, outs, 1, groups, se),
+                          {(const char*)x.zeros, (const char*)x.zeros + (x.zeros ? (x.out_dim - 1L) * x.zeros_pitch + groups : 0)}, {(const char*)x.bias, (const char*)x.bias + (x.bias ? (long)x.out_dim * e : 0)}};
+    for (const OpSpan& i : in) if (op_meet(o, i)) return set_err(DPDF_E_INVALID, "w4 matvec: out overlaps an input");
+    OpDevice dev(device);
+    HIP_TRY(dev.err);
+    W4Args a{x.x, x.x_stride, x.codes, x.codes_pitch, x.scales, x.scales_stride, x.zeros, x.zeros_pitch, x.bias, x.out, x.out_stride, x.rows, x.in_dim, x.out_dim, x.group};
+    if ((x.rows + 7L) / 8 > 65535) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
+    const dim3 grid((unsigned)((x.out_dim + 3L) / 4), (unsigned)((x.rows + 7L) / 8));
+    gd_types(x.dtype, x.scale_dtype, [&](auto t, auto g) { w4_matvec_any_kernel<decltype(t), decltype(g)><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+    HIP_TRY(hipGetLastError());
+    return DPDF_OK;
+}

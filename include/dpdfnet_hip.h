@@ -204,6 +204,66 @@ int dpdf_set_option(dpdf_model* m, const char* name, int value);
 long dpdf_resample_len(long n_in, int sr_in, int sr_out);      /* ceil(n_in * sr_out / sr_in); -1 on bad arguments */
 int dpdf_resample(int device, const float* in, int B, long n_in, int sr_in, int sr_out, float* out, int flags);
 
+/* ------------------------------------------------------------------------------------------------------------------------------
+ * Stand-alone operators: device pointers only, on `device` and the caller's `stream` (a hipStream_t, NULL = the default stream);
+ * nothing is allocated and nothing waited for, so every call can be captured into a graph.  Arguments are checked before anything
+ * is launched.  Strides count elements, pitches bytes; the last dimension is contiguous.  An output may not overlap an input or
+ * itself.  Values that are no dpdf_dtype, sizes out of range, overlaps: DPDF_E_INVALID. */
+enum { DPDF_F32 = 0, DPDF_F16 = 1, DPDF_BF16 = 2 };
+
+/* The gated delta rule, a recurrence over frames with a matrix state S [k_dim][v_dim] per sequence and value head:
+ *   S' = exp(g_t) S_{t-1};  e_t = beta_t (v_t - S'^T k_t);  S_t = S' + k_t e_t^T;  out_t = scale S_t^T q_t
+ * q, k [batch, frames, k_heads, k_dim]; v, out [batch, frames, v_heads, v_dim]; g, beta [batch, frames, v_heads];
+ * state_in, state_out [batch, v_heads, k_dim, v_dim] fp32, contiguous.  k_dim 1 .. 128; v_heads a multiple of k_heads, value head h reads
+ * key head h / (v_heads / k_heads).  The state is held, and every sum taken, in fp32.  g = -inf resets the state. */
+typedef struct dpdf_gated_delta_args {
+    int dtype, gate_dtype;                   /* of q, k, v, out; of g, beta: DPDF_F32 or dtype */
+    int batch, frames, k_heads, v_heads, k_dim, v_dim;
+    float scale;
+    const void *q, *k, *v, *g, *beta;
+    void* out;
+    long q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3], out_stride[3];      /* batch, frame, head */
+    const float* state_in;                   /* clips: NULL = zeros */
+    float* state_out;                        /* may be state_in itself; clips: NULL = not wanted */
+    const int* lengths;                      /* clips: device [batch], frames of each (held to 0 .. frames), NULL = all */
+    const unsigned char* active;             /* steps: device [batch], 0 = this stream is left out, NULL = all */
+} dpdf_gated_delta_args;
+
+/* Whole clips, in chunks of 64 frames.  Frames behind a clip's length are neither read nor written; state_out is the state after its last
+ * frame (a clip of length 0: the state it came with).  A non-finite k, g (but -inf) or beta makes the outputs of its head from its frame
+ * on, and its state, NaN, a non-finite v those of its column, a non-finite q those of its frame; nothing earlier and no other head. */
+int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* stream);
+/* `frames` hops (one, or a few) of every active stream, frame by frame; state_in is required, state_out = state_in updates it in place.
+ * Rows of streams that are left out are neither read nor written. */
+int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* args, void* stream);
+
+/* Dense layers with 4-bit weights: out[m][n] = sum_k x[m][k] (code[n][k] - zero[n][k / group]) scale[n][k / group] + bias[n], sums in fp32.
+ * Codes are two to a byte, the lower half first (codes [out_dim, (in_dim + 1) / 2]); scales, zeros [out_dim, ceil(in_dim / group)];
+ * group a multiple of 32, the last one may be short. */
+typedef struct dpdf_w4_matvec_args {
+    int dtype, scale_dtype;                  /* of x, bias, out; of scales: DPDF_F32 or dtype */
+    int rows, in_dim, out_dim, group;
+    const void* x; long x_stride;
+    const unsigned char* codes; long codes_pitch;
+    const void* scales; long scales_stride;
+    const unsigned char* zeros; long zeros_pitch;      /* NULL = 8 */
+    const void* bias;                        /* NULL = none */
+    void* out; long out_stride;
+} dpdf_w4_matvec_args;
+int dpdf_w4_matvec(int device, const dpdf_w4_matvec_args* args, void* stream);
+
+/* Codes, scales (and zeros, if not NULL) of a weight matrix [out_dim, in_dim].  With zeros a group's range, 0 included, is divided into 15
+ * steps, without them its largest magnitude into 7; codes are the nearest (ties to even) under the scale as it is stored. */
+typedef struct dpdf_w4_quantize_args {
+    int dtype;                               /* of weight and scales */
+    int in_dim, out_dim, group;
+    const void* weight; long weight_stride;
+    unsigned char* codes; long codes_pitch;
+    void* scales; long scales_stride;
+    unsigned char* zeros; long zeros_pitch;
+} dpdf_w4_quantize_args;
+int dpdf_w4_quantize(int device, const dpdf_w4_quantize_args* args, void* stream);
+
 /* Debug/test hook: copy an intermediate tensor of the last processed chunk to the host
  * ("e0","e1","e2","e3","e3_dprnn","c0","c1","c1_dprnn","emb","m","coefs","xm","feat_erb",
  * "feat_spec"; engine-native channels-last layouts).  Returns the element count, -1 if unknown. */

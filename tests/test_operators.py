@@ -1,0 +1,721 @@
+"""The stand-alone operators (`dpdfnet_amd.operators`): gated delta rule over clips and hop by hop, dense layers with 4-bit weights.
+CPU: refusals, argument layouts, the alias.  GPU: every form against its definition in 64 bits.
+
+Tolerances.  u = 2^-24 is half a step of fp32.  A frame of the recurrence takes sums of Dk products and a chunk sums of 64 more; with |k| <= 1 and
+0 <= beta <= 1 a frame's error is not amplified later, so after T frames at most T (Dk + 64) roundings of relative size u have added up,
+like a random walk: TOL = 8 deviations = 8 sqrt(T (Dk + 64)) u of the largest magnitude.  On top comes the result's own rounding, half a step of
+its type relative to the value (bf16 2^-8, fp16 2^-11)."""
+import ctypes
+import math
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from dpdfnet_amd import backend, operators
+
+ROOT = Path(__file__).resolve().parents[1]
+U = 2.0 ** -24
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -24, torch.bfloat16: 2.0 ** -133}
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# definitions in 64 bits, on the CPU
+# ---------------------------------------------------------------------------------------------------------------------------------------
+def delta_rule(q, k, v, g, beta, state=None, lengths=None, scale=None):
+    q, k, v, g, beta = (t.detach().double().cpu() for t in (q, k, v, g, beta))
+    B, T, Hk, Dk = q.shape
+    Hv, Dv = v.shape[2:]
+    head = torch.arange(Hv) // (Hv // Hk)
+    q, k = q[:, :, head], k[:, :, head]
+    scale = 1 / math.sqrt(Dk) if scale is None else scale
+    S = torch.zeros(B, Hv, Dk, Dv, dtype=torch.float64) if state is None else state.detach().double().cpu().clone()
+    out = torch.zeros(B, T, Hv, Dv, dtype=torch.float64)
+    n = torch.full((B,), T) if lengths is None else lengths.cpu().long()
+    for t in range(T):
+        on = (t < n)[:, None, None]
+        Sd = S * g[:, t].exp()[..., None, None]
+        e = beta[:, t, :, None] * (v[:, t] - (Sd * k[:, t, :, :, None]).sum(2))
+        new = Sd + k[:, t, :, :, None] * e[:, :, None]
+        out[:, t] = torch.where(on, scale * (new * q[:, t, :, :, None]).sum(2), out[:, t])
+        S = torch.where(on[..., None], new, S)
+    return out, S
+
+
+def w4_layer(x, codes, scales, zeros, bias, group):
+    x, codes, scales = x.detach().double().cpu(), codes.cpu(), scales.double().cpu()
+    K = x.shape[-1]
+    k = torch.arange(K)
+    c = ((codes[:, k // 2].int() >> (4 * (k % 2))) & 15).double()
+    z = 8.0 if zeros is None else zeros.cpu().double()[:, k // group]
+    w = (c - z) * scales[:, k // group]
+    y = x @ w.t()
+    return (y if bias is None else y + bias.double().cpu()), x.abs() @ w.abs().t()
+
+
+def inputs(B, T, Hk, Hv, Dk, Dv, dtype, seed=0, device="cuda", g_std=1.0):
+    gen = torch.Generator().manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, generator=gen)
+    q, k = (torch.nn.functional.normalize(r(B, T, Hk, Dk), dim=-1).to(dtype) for _ in range(2))
+    g = -torch.rand(B, T, Hv, generator=gen) * torch.exp(g_std * r(Hv) - 2)
+    return [t.to(device) for t in (q, k, r(B, T, Hv, Dv).to(dtype), g, torch.sigmoid(r(B, T, Hv)))]
+
+
+def tol(T, Dk):
+    return 8 * math.sqrt(T * (Dk + 64)) * U
+
+
+def near(got, ref, rel, half_step=0.0, tiny=0.0):
+    """|got - ref| <= rel * (largest |ref|) + half a step of the result's type."""
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape
+    top = float(ref.abs().max()) if ref.numel() else 0.0
+    bound = rel * top + half_step * ref.abs() * (1 + rel) + tiny
+    off = (got - ref).abs()
+    assert torch.isfinite(got).all()
+    assert bool((off <= bound).all()), f"worst {float((off / bound.clamp_min(1e-300)).max()):.3g} of the bound"
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# CPU
+# ---------------------------------------------------------------------------------------------------------------------------------------
+def test_argument_structures_match_the_header(tmp_path):
+    pairs = {"dpdf_gated_delta_args": operators._GatedDeltaArgs, "dpdf_w4_matvec_args": operators._W4MatvecArgs, "dpdf_w4_quantize_args": operators._W4QuantizeArgs}
+    src = '#include <stdio.h>\n#include <stddef.h>\n#include "dpdfnet_hip.h"\nint main(void) {\n'
+    for name, cls in pairs.items():
+        src += f'printf("{name} %zu", sizeof({name}));' + "".join(f'printf(" %zu", offsetof({name}, {f[0]}));' for f in cls._fields_) + 'printf("\\n");\n'
+    (tmp_path / "s.c").write_text(src + "return 0; }\n")
+    subprocess.run(["gcc", "-I" + str(ROOT / "include"), "-o", str(tmp_path / "s"), str(tmp_path / "s.c")], check=True)
+    for line in subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.splitlines():
+        name, *nums = line.split()
+        cls = pairs[name]
+        assert [int(n) for n in nums] == [ctypes.sizeof(cls)] + [getattr(cls, f[0]).offset for f in cls._fields_]
+
+
+def test_operators_are_reachable_under_both_names():
+    import dpdfnet.operators as alias
+    assert alias is operators
+    assert set(operators.__all__) == {"gated_delta", "gated_delta_step", "w4_matvec", "w4_quantize"}
+
+
+def _c_gated(step=False, **change):
+    """A call of the C entry on made-up addresses with one thing changed: refused before any of them is looked at."""
+    B, T, Hk, Hv, Dk, Dv = 2, 3, 2, 4, 16, 8
+    v = dict(dtype=2, gate_dtype=0, batch=B, frames=T, k_heads=Hk, v_heads=Hv, k_dim=Dk, v_dim=Dv, scale=1.0,
+             q=0x1000000, k=0x2000000, v=0x3000000, g=0x4000000, beta=0x5000000, out=0x6000000,
+             q_stride=(T * Hk * Dk, Hk * Dk, Dk), k_stride=(T * Hk * Dk, Hk * Dk, Dk), v_stride=(T * Hv * Dv, Hv * Dv, Dv),
+             g_stride=(T * Hv, Hv, 1), beta_stride=(T * Hv, Hv, 1), out_stride=(T * Hv * Dv, Hv * Dv, Dv),
+             state_in=0x7000000, state_out=0x7000000, lengths=None, active=None)
+    v.update(change)
+    a = operators._GatedDeltaArgs(*[v[f[0]] for f in operators._GatedDeltaArgs._fields_])
+    L = backend.load_library()
+    rc = (L.dpdf_gated_delta_step if step else L.dpdf_gated_delta)(0, ctypes.addressof(a), None)
+    return rc, L.dpdf_last_error().decode()
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(dtype=3), "dtypes"), (dict(dtype=-1), "dtypes"), (dict(gate_dtype=1), "dtypes"), (dict(batch=-1), "negative"), (dict(frames=-1), "negative"),
+    (dict(k_heads=3), "multiple"), (dict(k_heads=0), "multiple"), (dict(v_heads=0), "multiple"), (dict(k_dim=0), "head sizes"), (dict(k_dim=129), "head sizes"),
+    (dict(v_dim=0), "head sizes"), (dict(scale=float("nan")), "finite"), (dict(scale=float("inf")), "finite"), (dict(q=None), "null"), (dict(out=None), "null"),
+    (dict(v=0x3000001), "aligned"), (dict(g=0x4000002), "aligned"), (dict(state_in=0x7000002, state_out=None), "aligned"), (dict(lengths=0x8000001), "aligned"),
+    (dict(q_stride=(-1, 1, 1)), "negative stride"), (dict(out_stride=(0, 32, 8)), "share"), (dict(out_stride=(96, 32, 7)), "share"), (dict(out_stride=(96, 24, 8)), "share"),
+    (dict(out=0x3000000), "overlaps an input"), (dict(out=0x1000000 - 2), "overlaps an input"), (dict(out=0x7000000), "out overlaps"),
+    (dict(state_out=0x7000004), "in part"), (dict(state_out=0x2000000), "overlaps an input"), (dict(active=0x9000000), "mask"),
+    (dict(batch=1 << 30), "too large"),
+])
+def test_gated_delta_refusals(change, word):
+    rc, msg = _c_gated(**change)
+    assert rc == -1 and word in msg, (rc, msg)
+
+
+def test_gated_delta_step_refusals_and_empty_calls():
+    assert _c_gated(step=True, lengths=0x8000000)[0] == -1
+    assert _c_gated(step=True, state_in=None)[0] == -1 and _c_gated(step=True, state_out=None)[0] == -1
+    L = backend.load_library()
+    assert L.dpdf_gated_delta(0, None, None) == -1 and L.dpdf_gated_delta_step(0, None, None) == -1
+    assert L.dpdf_w4_matvec(0, None, None) == -1 and L.dpdf_w4_quantize(0, None, None) == -1
+    # nothing to do: no device is touched
+    assert _c_gated(batch=0)[0] == 0 and _c_gated(step=True, batch=0)[0] == 0 and _c_gated(step=True, frames=0)[0] == 0
+    assert _c_gated(frames=0, state_out=None)[0] == 0
+    if backend.device_count() == 0:
+        assert _c_gated()[0] == -2 and _c_gated(step=True)[0] == -2        # no GPU: a failure, nothing computed elsewhere
+
+
+def _c_w4(**change):
+    v = dict(dtype=1, scale_dtype=1, rows=2, in_dim=100, out_dim=6, group=32, x=0x1000000, x_stride=100, codes=0x2000000, codes_pitch=50,
+             scales=0x3000000, scales_stride=4, zeros=0x4000000, zeros_pitch=4, bias=0x5000000, out=0x6000000, out_stride=6)
+    v.update(change)
+    a = operators._W4MatvecArgs(*[v[f[0]] for f in operators._W4MatvecArgs._fields_])
+    L = backend.load_library()
+    return L.dpdf_w4_matvec(0, ctypes.addressof(a), None), L.dpdf_last_error().decode()
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(dtype=9), "dtype"), (dict(scale_dtype=2), "dtypes"), (dict(rows=-1), "negative"), (dict(in_dim=0), "empty"), (dict(out_dim=0), "empty"),
+    (dict(group=0), "group"), (dict(group=48), "group"), (dict(group=-32), "group"), (dict(x=None), "null"), (dict(codes=None), "null"), (dict(scales=None), "null"),
+    (dict(out=None), "null"), (dict(x_stride=-1), "negative stride"), (dict(out_stride=5), "share"), (dict(x=0x1000001), "aligned"), (dict(scales=0x3000001), "aligned"),
+    (dict(out=0x1000000), "overlaps"), (dict(out=0x2000020), "overlaps"), (dict(out=0x3000000), "overlaps"), (dict(out=0x4000000), "overlaps"), (dict(out=0x5000002), "overlaps"),
+])
+def test_w4_refusals(change, word):
+    rc, msg = _c_w4(**change)
+    assert rc == -1 and word in msg, (rc, msg)
+
+
+def test_w4_empty_call_and_quantize_refusals():
+    assert _c_w4(rows=0)[0] == 0
+    base = dict(dtype=0, in_dim=100, out_dim=6, group=32, weight=0x1000000, weight_stride=100, codes=0x2000000, codes_pitch=50,
+                scales=0x3000000, scales_stride=4, zeros=0x4000000, zeros_pitch=4)
+    L = backend.load_library()
+    for change in (dict(dtype=5), dict(in_dim=0), dict(group=16), dict(weight=None), dict(codes=None), dict(scales=None), dict(codes_pitch=49), dict(scales_stride=3),
+                   dict(zeros_pitch=3), dict(weight_stride=-1), dict(weight=0x1000002), dict(scales=0x1000004), dict(codes=0x3000000), dict(zeros=0x2000010)):
+        v = {**base, **change}
+        a = operators._W4QuantizeArgs(*[v[f[0]] for f in operators._W4QuantizeArgs._fields_])
+        assert L.dpdf_w4_quantize(0, ctypes.addressof(a), None) == -1, change
+
+
+def test_python_layer_refuses_what_is_on_the_cpu_or_of_a_wrong_kind():
+    q, k, v, g, beta = inputs(1, 2, 1, 2, 16, 16, F32, device="cpu")
+    state = torch.zeros(1, 2, 16, 16)
+    with pytest.raises(ValueError, match="GPU"):
+        operators.gated_delta(q, k, v, g, beta)
+    with pytest.raises(ValueError, match="GPU"):
+        operators.gated_delta_step(q, k, v, g, beta, state)
+    with pytest.raises(ValueError, match="state"):
+        operators.gated_delta_step(q, k, v, g, beta, None)
+    with pytest.raises(ValueError, match="tensor"):
+        operators.gated_delta([1.0], k, v, g, beta)
+    with pytest.raises(ValueError, match="dimensions"):
+        operators.gated_delta(q[0], k, v, g, beta)
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        operators.gated_delta(q.double(), k, v, g, beta)
+    with pytest.raises(ValueError, match="GPU"):
+        operators.w4_matvec(torch.zeros(2, 64), torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 1))
+    with pytest.raises(ValueError, match="group"):
+        operators.w4_matvec(torch.zeros(2, 64), torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 1), group=40)
+    with pytest.raises(ValueError, match="GPU"):
+        operators.w4_quantize(torch.zeros(4, 64))
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# GPU: the gated delta rule
+# ---------------------------------------------------------------------------------------------------------------------------------------
+CLIPS = [  # B, T, Hk, Hv, Dk, Dv
+    (1, 1, 1, 1, 16, 16), (2, 2, 1, 1, 1, 1), (1, 16, 1, 2, 17, 33), (2, 63, 2, 2, 32, 16), (1, 64, 1, 3, 64, 64), (3, 65, 2, 4, 64, 48),
+    (1, 127, 1, 1, 128, 128), (2, 130, 3, 3, 48, 100), (1, 257, 2, 6, 80, 17), (1, 400, 1, 2, 128, 64), (5, 70, 1, 1, 5, 130),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", CLIPS)
+def test_clips_against_the_definition(shape, dtype):
+    B, T, Hk, Hv, Dk, Dv = shape
+    x = inputs(*shape, dtype, seed=T)
+    state = 0.5 * torch.randn(B, Hv, Dk, Dv, generator=torch.Generator().manual_seed(1)).cuda()
+    for s in (None, state):
+        out, end = operators.gated_delta(*x, state=s)
+        ref, rend = delta_rule(*x, state=s)
+        near(out, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
+        near(end, rend, tol(T, Dk))
+    assert torch.equal(state, 0.5 * torch.randn(B, Hv, Dk, Dv, generator=torch.Generator().manual_seed(1)).cuda())        # read only
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 16, 16), (2, 3, 1, 2, 1, 1), (3, 1, 2, 6, 17, 33), (4, 2, 1, 1, 64, 64), (2, 4, 2, 4, 128, 128), (1, 5, 1, 2, 100, 30),
+                                   (7, 1, 4, 4, 48, 40)])
+def test_steps_against_the_definition(shape, dtype):
+    B, T, Hk, Hv, Dk, Dv = shape
+    x = inputs(*shape, dtype, seed=B)
+    state = 0.5 * torch.randn(B, Hv, Dk, Dv, generator=torch.Generator().manual_seed(1)).cuda()
+    ref, rend = delta_rule(*x, state=state)
+    ptr = state.data_ptr()
+    out = operators.gated_delta_step(*x, state)
+    assert state.data_ptr() == ptr
+    near(out, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
+    near(state, rend, tol(T, Dk))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gates_of_the_values_type(dtype):
+    x = inputs(2, 100, 2, 2, 32, 32, dtype, seed=4)
+    x[3], x[4] = x[3].to(dtype), x[4].to(dtype)
+    out, end = operators.gated_delta(*x)
+    ref, rend = delta_rule(*x)
+    near(out, ref, tol(100, 32), HALF_STEP[dtype], TINY[dtype])
+    near(end, rend, tol(100, 32))
+    state = torch.zeros(2, 2, 32, 32, device="cuda")
+    out = operators.gated_delta_step(*[t[:, :3] for t in x], state)
+    ref, rend = delta_rule(*[t[:, :3] for t in x])
+    near(out, ref, tol(3, 32), HALF_STEP[dtype], TINY[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [64, 128])
+def test_hard_gates_and_keys(dtype, D):
+    """No decay, decays that empty the state within a frame, resets by -inf, beta of 0 and 1, and one key in every frame."""
+    T = 150
+    q, k, v, g, beta = inputs(1, T, 1, 6, D, 32, dtype, seed=9)
+    g = g.clone()
+    g[:, :, 0] = 0
+    g[:, :, 1] = -30
+    g[:, ::37, 2] = -math.inf
+    g[:, :, 3] = torch.where(torch.rand(1, T, generator=torch.Generator().manual_seed(2)).cuda() < 0.5, -100.0, -0.001)
+    beta = beta.clone()
+    beta[:, ::2, 4] = 0
+    beta[:, :, 0] = 1
+    for keys in (k, k[:, :1].expand(-1, T, -1, -1), torch.zeros_like(k)):
+        out, end = operators.gated_delta(q, keys, v, g, beta)
+        ref, rend = delta_rule(q, keys, v, g, beta)
+        near(out, ref, tol(T, D), HALF_STEP[dtype], TINY[dtype])
+        near(end, rend, tol(T, D))
+        state = torch.zeros(1, 6, D, 32, device="cuda")
+        out = operators.gated_delta_step(q[:, :40], keys[:, :40], v[:, :40], g[:, :40], beta[:, :40], state)
+        near(out, ref[:, :40], tol(40, D), HALF_STEP[dtype], TINY[dtype])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [(0, 0, 0), (1, 64, 0), (65, 130, 3), (130, 129, 128), (-5, 1000, 66)])
+def test_ragged_clips_leave_the_rest_alone(lens):
+    B, T, dtype = 3, 130, BF16
+    x = inputs(B, T, 1, 2, 32, 48, dtype, seed=3)
+    held = torch.tensor([min(max(n, 0), T) for n in lens])
+    for b in range(B):                        # nothing behind the end may be looked at
+        for t in x:
+            t[b, held[b]:] = math.nan
+    state = torch.randn(B, 2, 32, 48, generator=torch.Generator().manual_seed(1)).cuda()
+    out = torch.full((B, T, 2, 48), 7.0, device="cuda", dtype=dtype)
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    got, end = operators.gated_delta(*x, state=state, lengths=lengths, out=out)
+    assert got is out
+    ref, rend = delta_rule(*[torch.nan_to_num(t, nan=0.0) for t in x], state=state, lengths=held)
+    on = (torch.arange(T)[None] < held[:, None])[..., None, None].expand_as(ref)
+    assert bool((out.cpu()[~on] == 7.0).all())
+    if bool(on.any()):
+        near(torch.where(on, out.cpu().double(), 0.0), ref, tol(T, 32), HALF_STEP[dtype], TINY[dtype])
+    near(end, rend, tol(T, 32))
+    for b in range(B):
+        if held[b] == 0:
+            assert torch.equal(end[b], state[b])
+    assert bool((operators.gated_delta(*x, lengths=lengths)[0].cpu()[~on] == 0).all())
+
+
+@pytest.mark.gpu
+def test_clips_without_a_frame():
+    x = inputs(2, 4, 1, 1, 16, 16, F32)
+    none = [t[:, :0] for t in x]
+    state = torch.randn(2, 1, 16, 16, device="cuda")
+    out, end = operators.gated_delta(*none, state=state)
+    assert out.shape == (2, 0, 1, 16) and torch.equal(end, state)
+    out, end = operators.gated_delta(*none)
+    assert bool((end == 0).all())
+    before = state.clone()
+    assert operators.gated_delta_step(*none, state).shape == (2, 0, 1, 16) and torch.equal(state, before)
+    out, end = operators.gated_delta(*[t[:0] for t in x])
+    assert out.shape == (0, 4, 1, 16) and end.shape == (0, 1, 16, 16)
+
+
+@pytest.mark.gpu
+def test_streams_left_out_keep_their_rows():
+    S, T, dtype = 6, 2, F16
+    x = inputs(S, T, 2, 2, 32, 32, dtype, seed=5)
+    on = torch.tensor([1, 0, 1, 1, 0, 0], dtype=torch.uint8)
+    for t in x:
+        t[on == 0] = math.nan
+    state = torch.randn(S, 2, 32, 32, generator=torch.Generator().manual_seed(1)).cuda()
+    state[1] = math.inf
+    ref, rend = delta_rule(*[t[(on == 1).cuda()] for t in x], state=state[(on == 1).cuda()])
+    for mask in (on, on.bool()):
+        s, out = state.clone(), torch.full((S, T, 2, 32), 7.0, device="cuda", dtype=dtype)
+        operators.gated_delta_step(*x, s, active=mask.cuda(), out=out)
+        assert bool((out[(on == 0).cuda()] == 7.0).all()) and torch.equal(s[(on == 0).cuda()], state[(on == 0).cuda()])
+        near(out[(on == 1).cuda()], ref, tol(T, 32), HALF_STEP[dtype], TINY[dtype])
+        near(s[(on == 1).cuda()], rend, tol(T, 32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_any_strides(dtype):
+    B, T, H, D = 2, 90, 2, 32
+    q, k, v, g, beta = inputs(B, T, H, H, D, D, dtype, seed=6)
+    ref, rend = operators.gated_delta(q, k, v, g, beta)
+    fused = torch.cat((q, k, v), dim=-1)                                     # one projection's output, three views of it
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+    frames_first = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, k, v)]
+    wide = torch.zeros(B, T, H, D + 3, device="cuda", dtype=dtype)           # rows at odd addresses
+    odd = []
+    for t in (q, k, v):
+        w = wide.clone()
+        w[..., 1:D + 1] = t
+        odd.append(w[..., 1:D + 1])
+    gates = [t.permute(2, 0, 1).contiguous().permute(1, 2, 0) for t in (g, beta)]
+    for views in ([fused[..., :D], fused[..., D:2 * D], fused[..., 2 * D:]], heads_first, frames_first, odd):
+        out = torch.zeros(B, H, T, 2 * D, device="cuda", dtype=dtype)
+        got, end = operators.gated_delta(*views, *gates, out=out.transpose(1, 2)[..., :D])
+        assert torch.equal(got, ref) and torch.equal(end, rend)
+        assert bool((out[..., D:] == 0).all())
+        s, s2 = torch.zeros_like(rend), torch.zeros_like(rend)
+        a = operators.gated_delta_step(*[t[:, :3] for t in views], gates[0][:, :3], gates[1][:, :3], s)
+        b = operators.gated_delta_step(q[:, :3], k[:, :3], v[:, :3], g[:, :3], beta[:, :3], s2)
+        assert torch.equal(a, b) and torch.equal(s, s2)
+    same = [t[:1].expand(B, -1, -1, -1) for t in (q, k, v)] + [t[:1].expand(B, -1, -1) for t in (g, beta)]
+    out, end = operators.gated_delta(*same)                                  # one clip for every row of the batch: bit-identical rows
+    assert torch.equal(out[0], out[1]) and torch.equal(end[0], end[1]) and torch.equal(out[0], ref[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cut", [1, 64, 100, 150])
+def test_a_clip_in_two_calls_and_clip_against_steps(dtype, cut):
+    x = inputs(2, 180, 2, 4, 64, 32, dtype, seed=8)
+    ref, rend = delta_rule(*x)
+    o1, s = operators.gated_delta(*[t[:, :cut] for t in x])
+    o2, s2 = operators.gated_delta(*[t[:, cut:] for t in x], state=s, state_out=s)
+    assert s2 is s
+    near(torch.cat((o1, o2), 1), ref, tol(180, 64), HALF_STEP[dtype], TINY[dtype])
+    near(s, rend, tol(180, 64))
+    s = torch.zeros_like(s)
+    o = torch.cat([operators.gated_delta_step(*[t[:, i:i + 60] for t in x], s) for i in range(0, 180, 60)], 1)
+    near(o, ref, tol(180, 64), HALF_STEP[dtype], TINY[dtype])
+    near(s, rend, tol(180, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("what, at", [("q", 70), ("k", 70), ("v", 70), ("g", 70), ("beta", 70), ("k", 0), ("v", 127), ("k", 129)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_a_non_finite_value_stays_where_it_belongs(dtype, what, at, value):
+    x = inputs(2, 130, 2, 2, 32, 32, dtype, seed=11)
+    clean, cend = operators.gated_delta(*x)
+    y = [t.clone() for t in x]
+    t = y["q k v g beta".split().index(what)]
+    if what in ("g", "beta"):
+        t[1, at, 0] = value
+    else:
+        t[1, at, 0, 5] = value
+    out, end = operators.gated_delta(*y)
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    if what == "q":
+        hit[1, at, 0] = True
+    elif what == "v":
+        hit[1, at:, 0, 5] = True
+    else:
+        hit[1, at:, 0] = True
+    assert torch.equal(out[~hit], clean[~hit])                # other clips, heads and earlier frames: bit for bit
+    assert not bool(torch.isfinite(out[hit]).any())
+    shit = torch.zeros_like(end, dtype=torch.bool)
+    if what == "v":
+        shit[1, 0, :, 5] = True
+    elif what != "q":
+        shit[1, 0] = True
+    assert torch.equal(end[~shit], cend[~shit]) and not bool(torch.isfinite(end[shit]).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_large_and_small_values_keep_their_precision(dtype):
+    """Rows of v and states of very different size side by side: each column is as exact as it would be alone."""
+    q, k, v, g, beta = inputs(1, 100, 1, 1, 64, 64, dtype, seed=12)
+    size = 2.0 ** torch.linspace(-8, 8, 64).round().cuda()
+    state = torch.randn(1, 1, 64, 64, generator=torch.Generator().manual_seed(1)).cuda() * size
+    v = (v * size).to(dtype)
+    out, end = operators.gated_delta(q, k, v, g, beta, state=state)
+    ref, rend = delta_rule(q, k, v, g, beta, state=state)
+    for c in range(64):
+        near(out[..., c], ref[..., c], tol(100, 64), HALF_STEP[dtype], TINY[dtype])
+        near(end[..., c], rend[..., c], tol(100, 64))
+
+
+@pytest.mark.gpu
+def test_scale_is_the_callers():
+    x = inputs(1, 70, 1, 1, 32, 32, F32)
+    s = torch.zeros(1, 1, 32, 32, device="cuda")
+    for scale in (0.0, 1.0, -2.5):
+        ref, _ = delta_rule(*x, scale=scale)
+        near(operators.gated_delta(*x, scale=scale)[0], ref, tol(70, 32))
+        near(operators.gated_delta_step(*[t[:, :2] for t in x], s.clone(), scale=scale), ref[:, :2], tol(70, 32))
+
+
+@pytest.mark.gpu
+def test_refusals_of_device_tensors():
+    q, k, v, g, beta = inputs(2, 8, 1, 2, 32, 32, BF16)
+    state = torch.zeros(2, 2, 32, 32, device="cuda")
+    bad = [dict(k=k[..., :16]), dict(k=k.float()), dict(v=v[:1]), dict(g=g.half()), dict(beta=beta.bfloat16()), dict(g=g[:, :, :1]), dict(state=state.half()),
+           dict(state=state.transpose(2, 3)), dict(state=state[:1]), dict(lengths=torch.tensor([1, 2], device="cuda")), dict(lengths=torch.tensor([1, 2], dtype=torch.int32)),
+           dict(out=torch.zeros(2, 8, 2, 32, device="cuda")), dict(out=v), dict(q=q.transpose(1, 3).contiguous().transpose(1, 3)), dict(scale=math.nan)]
+    good = dict(q=q, k=k, v=v, g=g, beta=beta)
+    for change in bad:
+        with pytest.raises(ValueError):
+            operators.gated_delta(**{**good, **change})
+    with pytest.raises(ValueError, match="gradient"):
+        operators.gated_delta(q, k, v.clone().requires_grad_(), g, beta)
+    with torch.no_grad():
+        operators.gated_delta(q, k, v.clone().requires_grad_(), g, beta)
+    with pytest.raises(ValueError):
+        operators.gated_delta_step(q, k, v, g, beta, state, active=torch.ones(2, device="cuda"))
+    with pytest.raises(ValueError, match="head sizes"):
+        operators.gated_delta(*inputs(1, 4, 1, 1, 144, 16, F32))
+    both = torch.zeros(2 * 2 * 2 * 32 * 32, device="cuda")
+    with pytest.raises(ValueError, match="in part"):
+        operators.gated_delta(q, k, v, g, beta, state=both[:4096].view(2, 2, 32, 32), state_out=both[16:4112].view(2, 2, 32, 32))
+    x, codes, scales = torch.zeros(2, 64, device="cuda"), torch.zeros(4, 32, dtype=torch.uint8, device="cuda"), torch.zeros(4, 1, device="cuda")
+    for change in (dict(codes=codes[:, :31]), dict(scales=scales.half()), dict(scales=scales[:, :0]), dict(zeros=scales), dict(bias=scales), dict(out=x), dict(codes=codes.int())):
+        with pytest.raises(ValueError):
+            operators.w4_matvec(**{**dict(x=x, codes=codes, scales=scales), **change})
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    far = 2 ** 31 + 64
+    q, k, v, g, beta = inputs(2, 70, 1, 1, 32, 32, F16, seed=2)
+    buf = torch.zeros(far + 70 * 96, dtype=F16, device="cuda")
+    views = [buf.as_strided((2, 70, 1, 32), (far, 96, 32, 1), 32 * i) for i in range(3)]
+    for a, b in zip(views, (q, k, v)):
+        a.copy_(b)
+    obuf = torch.zeros(far + 70 * 32, dtype=F16, device="cuda")
+    ref, rend = operators.gated_delta(q, k, v, g, beta)
+    out, end = operators.gated_delta(*views, g, beta, out=obuf.as_strided((2, 70, 1, 32), (far, 32, 32, 1)))
+    assert torch.equal(out, ref) and torch.equal(end, rend)
+    s = torch.zeros_like(end)
+    s2 = s.clone()
+    assert torch.equal(operators.gated_delta_step(*[t[:, :2] for t in views], g[:, :2], beta[:, :2], s),
+                       operators.gated_delta_step(*[t[:, :2] for t in (q, k, v)], g[:, :2], beta[:, :2], s2)) and torch.equal(s, s2)
+    del buf, obuf, views, out
+    # a state of more than 2^31 values: the last stream's is right
+    S = 4100
+    x = inputs(1, 1, 1, 32, 128, 128, BF16, seed=3)
+    wide = [t.expand(S, *t.shape[1:]) for t in x]
+    state = torch.zeros(S, 32, 128, 128, device="cuda")
+    state[0] = state[-1] = 0.25
+    ref, rend = delta_rule(*x, state=state[-1:])
+    out = operators.gated_delta_step(*wide, state)
+    near(out[-1:], ref, tol(1, 128), HALF_STEP[BF16], TINY[BF16])
+    near(state[-1:], rend, tol(1, 128))
+    assert torch.equal(state[0], state[-1]) and torch.equal(out[0], out[-1])
+    end = operators.gated_delta(*wide, state=state, state_out=state)[1]
+    near(end[-1:], delta_rule(*x, state=rend.float())[1], 2 * tol(1, 128))
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# GPU: 4-bit layers
+# ---------------------------------------------------------------------------------------------------------------------------------------
+def layer(M, K, N, group, dtype, zeros, seed=0, scale_dtype=None):
+    gen = torch.Generator().manual_seed(seed)
+    groups = -(-K // group)
+    x = torch.randn(M, K, generator=gen).to(dtype).cuda()
+    codes = torch.randint(0, 256, (N, (K + 1) // 2), generator=gen, dtype=torch.uint8).cuda()
+    scales = (0.01 + torch.rand(N, groups, generator=gen)).to(scale_dtype or dtype).cuda()
+    z = torch.randint(0, 16, (N, groups), generator=gen, dtype=torch.uint8).cuda() if zeros else None
+    return x, codes, scales, z, torch.randn(N, generator=gen).to(dtype).cuda()
+
+
+def near_layer(y, ref, mag, K, dtype):
+    """A sum of K products and its pieces: 8 deviations of sqrt(K + 16) roundings of the magnitudes' sum, which bounds every partial sum; codes
+    with a zero of up to 15 may be taken apart into code and zero, which doubles the magnitudes at most threefold."""
+    bound = 8 * math.sqrt(K + 16) * U * 4 * mag + HALF_STEP[dtype] * ref.abs() * 1.01 + TINY[dtype]
+    off = (y.double().cpu() - ref).abs()
+    assert bool((off <= bound).all()), f"worst {float((off / bound).max()):.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M, K, N, group", [(1, 1, 1, 32), (1, 2, 3, 32), (2, 31, 17, 32), (1, 64, 64, 64), (3, 100, 50, 32), (1, 256, 768, 64), (4, 255, 33, 128), (7, 513, 100, 64),
+                                            (8, 1024, 96, 128), (9, 300, 31, 96), (16, 2048, 130, 32), (17, 640, 64, 640), (33, 333, 77, 64), (1, 8192, 48, 128), (5, 4096, 16, 4096),
+                                            (2, 160, 64, 1024)])
+def test_w4_layers_against_the_definition(M, K, N, group, dtype):
+    for zeros in (False, True):
+        x, codes, scales, z, bias = layer(M, K, N, group, dtype, zeros, seed=K + M)
+        for b in (None, bias):
+            ref, mag = w4_layer(x, codes, scales, z, b, group)
+            near_layer(operators.w4_matvec(x, codes, scales, zeros=z, bias=b, group=group), ref, mag, K, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_w4_strides_alignments_and_scale_types(dtype):
+    M, K, N, group = 5, 384, 70, 64
+    x, codes, scales, z, bias = layer(M, K, N, group, dtype, True, scale_dtype=F32)
+    ref, mag = w4_layer(x, codes, scales, z, bias, group)
+    near_layer(operators.w4_matvec(x, codes, scales, zeros=z, bias=bias, group=group), ref, mag, K, dtype)
+    near_layer(operators.w4_matvec(x[0], codes, scales, zeros=z, bias=bias, group=group), ref[0], mag[0], K, dtype)
+    near_layer(operators.w4_matvec(x[:1].expand(M, -1), codes, scales, zeros=z, bias=bias, group=group), ref[:1].expand(M, -1), mag[:1].expand(M, -1), K, dtype)
+    for off, pitch in ((0, 208), (1, 200), (4, 196), (8, 200), (16, 224)):
+        buf = torch.zeros(N * pitch + 32, dtype=torch.uint8, device="cuda")
+        c = buf.as_strided((N, K // 2), (pitch, 1), off)
+        c.copy_(codes)
+        xw = torch.zeros(M, K + 11, dtype=dtype, device="cuda")
+        xw[:, off % 8:off % 8 + K] = x
+        xw[:, off % 8 + K:] = math.nan                        # behind a row: never read
+        sw = torch.full((N, K // group + off), math.nan, device="cuda")
+        sw[:, off:] = scales
+        zw = torch.full((N, K // group + off), 99, dtype=torch.uint8, device="cuda")
+        zw[:, off:] = z
+        out = torch.full((M, N + 5), 7.0, dtype=dtype, device="cuda")
+        operators.w4_matvec(xw[:, off % 8:off % 8 + K], c, sw[:, off:], zeros=zw[:, off:], bias=bias, group=group, out=out[:, 2:N + 2])
+        near_layer(out[:, 2:N + 2], ref, mag, K, dtype)
+        assert bool((out[:, :2] == 7).all()) and bool((out[:, N + 2:] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M", [1, 6, 20])
+def test_w4_rows_are_independent_and_repeat(dtype, M):
+    x, codes, scales, z, _ = layer(M, 1000, 90, 128, dtype, True)
+    y = operators.w4_matvec(x, codes, scales, zeros=z, group=128)
+    assert torch.equal(y, operators.w4_matvec(x, codes, scales, zeros=z, group=128))
+    bad = x.clone()
+    bad[M - 1, 7], bad[M - 1, 900] = math.nan, math.inf
+    got = operators.w4_matvec(bad, codes, scales, zeros=z, group=128)
+    assert torch.equal(got[:M - 1], y[:M - 1]) and not bool(torch.isfinite(got[M - 1]).any())
+    s = scales.clone()
+    s[5, 2] = math.inf                                        # one output's weights
+    got = operators.w4_matvec(x, codes, s, zeros=z, group=128)
+    keep = torch.arange(90) != 5
+    assert torch.equal(got[:, keep], y[:, keep]) and not bool(torch.isfinite(got[:, 5]).any())
+
+
+@pytest.mark.gpu
+def test_w4_empty_batch_and_far_offsets():
+    x, codes, scales, z, bias = layer(3, 128, 40, 64, F16, False)
+    assert operators.w4_matvec(x[:0], codes, scales).shape == (0, 40)
+    buf = torch.zeros(2 * (2 ** 31 + 16) + 64, dtype=torch.uint8, device="cuda")        # rows of codes 2 GiB apart
+    c = buf.as_strided((3, 64), (2 ** 31 + 16, 1))
+    c.copy_(codes[:3])
+    assert torch.equal(operators.w4_matvec(x, c, scales[:3]), operators.w4_matvec(x, codes[:3].contiguous(), scales[:3]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("N, K, group", [(5, 64, 64), (33, 257, 32), (16, 1000, 128), (3, 1, 32), (64, 512, 4096)])
+def test_w4_quantize_is_the_formula(dtype, N, K, group):
+    gen = torch.Generator().manual_seed(K)
+    w = torch.randn(N, K, generator=gen).to(dtype)
+    w[0] = 0                                                  # a group of nothing
+    w[-1] = w[-1].abs()                                       # a group of one sign
+    if K > 60:
+        w[1, :14] = torch.arange(14).to(dtype) / 2 - 3.25     # ties
+    groups = -(-K // group)
+    pad = torch.nn.functional.pad(w.float(), [0, groups * group - K]).view(N, groups, group)
+    for symmetric in (False, True):
+        codes, scales, zeros = operators.w4_quantize(w.cuda(), group=group, symmetric=symmetric)
+        lo, hi = pad.amin(-1).clamp_max(0), pad.amax(-1).clamp_min(0)
+        s = (torch.maximum(hi, -lo) / 7 if symmetric else (hi - lo) / 15).to(dtype)
+        f = s.float()
+        z = torch.full_like(f, 8.0) if symmetric else torch.where(f > 0, (-lo / f).round().clamp(0, 15), 0.0)
+        c = torch.where(f[..., None] > 0, (pad / f[..., None]).round() + z[..., None], z[..., None]).clamp(0, 15).view(N, -1)[:, :K].to(torch.uint8)
+        assert scales.dtype == dtype and torch.equal(scales.cpu(), s)
+        assert (zeros is None) == symmetric and (symmetric or torch.equal(zeros.cpu().float(), z))
+        got = torch.stack((codes.cpu() & 15, codes.cpu() >> 4), -1).flatten(1)
+        assert codes.shape == (N, (K + 1) // 2) and codes.stride(0) % 16 == 0 and torch.equal(got[:, :K], c)
+        y, mag = w4_layer(torch.eye(K), codes, scales, zeros, None, group)
+        step = f.double().repeat_interleave(group, 1)[:, :K].t()
+        assert bool(((y - w.double().t()).abs() <= step * 0.5 * 1.1 + step * 8 * HALF_STEP[dtype] * 2).all())        # half a step, and the scale's own rounding over 8 to 15 steps
+
+
+# ---------------------------------------------------------------------------------------------------------------------------------------
+# GPU: together, on streams, in graphs
+# ---------------------------------------------------------------------------------------------------------------------------------------
+class Layer:
+    """A recurrent layer of a live stream as a program would build it: 4-bit projections of a frame to q, k, v and the gates, the recurrence, and a
+    4-bit projection back."""
+
+    def __init__(self, dtype, width=128, heads=2, dim=32, seed=0):
+        gen = torch.Generator().manual_seed(seed)
+        self.heads, self.dim, n = heads, dim, heads * dim
+        self.inw = (torch.randn(3 * n + 2 * heads, width, generator=gen) / math.sqrt(width)).to(dtype).cuda()
+        self.outw = (torch.randn(width, n, generator=gen) / math.sqrt(n)).to(dtype).cuda()
+        self.inq, self.outq = operators.w4_quantize(self.inw, group=32), operators.w4_quantize(self.outw, group=32)
+
+    def parts(self, y):
+        """[S, T, 3 n + 2 heads] -> q, k, v, g, beta"""
+        n = self.heads * self.dim
+        q, k, v = (y[..., i * n:(i + 1) * n].unflatten(-1, (self.heads, self.dim)) for i in range(3))
+        unit = [torch.nn.functional.normalize(t.float(), dim=-1).to(y.dtype) for t in (q, k)]
+        g, b = y[..., 3 * n:].float().chunk(2, -1)
+        return (*unit, v, -torch.nn.functional.softplus(g), torch.sigmoid(b))
+
+    def project(self, x, w):
+        return operators.w4_matvec(x.reshape(-1, x.shape[-1]), w[0], w[1], zeros=w[2], group=32).view(*x.shape[:-1], -1)
+
+    def clip(self, x):
+        o, s = operators.gated_delta(*self.parts(self.project(x, self.inq)))
+        return self.project(o.flatten(2), self.outq), s
+
+    def hop(self, x, state):
+        o = operators.gated_delta_step(*self.parts(self.project(x, self.inq)), state)
+        return self.project(o.flatten(2), self.outq)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_layer_over_clips_is_the_layer_hop_by_hop(dtype):
+    lay = Layer(dtype)
+    x = torch.randn(3, 70, 128, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    y, end = lay.clip(x)
+    state = torch.zeros_like(end)
+    hops = torch.cat([lay.hop(x[:, t:t + 1], state) for t in range(70)], 1)
+    # projections of one frame and of all are the same sums in one order or another; the recurrence's outputs are rounded to the type between
+    # the two projections, where one step's difference reaches the sums of 64 products
+    step = 2 * HALF_STEP[dtype]
+    near(hops, y.double().cpu(), 2 * tol(70, 32) + step, step)
+    near(state, end.double().cpu(), 2 * tol(70, 32) + (step if dtype != F32 else 0))
+    # and the whole against 64 bits, from the values that the codes stand for
+    (ci, si, zi), (co, so, zo) = lay.inq, lay.outq
+    p = w4_layer(x.flatten(0, 1), ci, si, zi, None, 32)[0].view(3, 70, -1).to(dtype).cuda()
+    o, rend = delta_rule(*lay.parts(p))
+    r = w4_layer(o.to(dtype).flatten(0, 1).flatten(1), co, so, zo, None, 32)[0].view(3, 70, -1)
+    near(y, r, 2 * tol(70, 32) + step, step)
+
+
+@pytest.mark.gpu
+def test_calls_on_other_streams_and_two_at_once():
+    lay = Layer(BF16)
+    xs = [torch.randn(2, 200, 128, generator=torch.Generator().manual_seed(i)).bfloat16().cuda() for i in range(2)]
+    want = [lay.clip(x) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(lay.clip(xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y, e in got[i]:
+            assert torch.equal(y, want[i][0]) and torch.equal(e, want[i][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_captured_calls_replay(dtype):
+    S = 5
+    lay = Layer(dtype)
+    x = torch.randn(S, 1, 128, device="cuda").to(dtype)
+    clip = torch.randn(2, 300, 128, device="cuda").to(dtype)
+    state = torch.zeros(S, 2, 32, 32, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        lay.hop(x, state.clone()); lay.clip(clip)
+    torch.cuda.current_stream().wait_stream(s)
+    g1, g2 = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g1):
+        y = lay.hop(x, state)
+    with torch.cuda.graph(g2):
+        yc, ec = lay.clip(clip)
+    mirror = torch.zeros_like(state)
+    state.zero_()
+    for r in range(4):
+        x.copy_(torch.randn(S, 1, 128, generator=torch.Generator().manual_seed(r)))
+        clip.copy_(torch.randn(2, 300, 128, generator=torch.Generator().manual_seed(50 + r)))
+        g1.replay(); g2.replay()
+        want, (wc, we) = lay.hop(x, mirror), lay.clip(clip)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(state, mirror) and torch.equal(yc, wc) and torch.equal(ec, we)
