@@ -99,6 +99,17 @@ template <typename F> void gd_types(int dtype, int gate, F f) {
     else { if (gate == DPDF_F32) f(__hip_bfloat16(), float()); else f(__hip_bfloat16(), __hip_bfloat16()); }
 }
 
+template <typename T, typename G>
+void w4_launch(const W4Args& a, hipStream_t s) {
+    const long tiles = ((long)a.N + 15) / 16, mt = ((long)a.M + 15) / 16;
+    const int nt = tiles * mt >= 1024 ? 2 : 1;
+    const int blocks = (a.K + 127) / 128, nw = blocks >= 8 ? 8 : blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+    const dim3 grid((unsigned)((tiles + nt - 1) / nt), (unsigned)mt);
+#define W4_RUN(R) (nt == 2 ? (w4_matvec_kernel<T, G, R, 2><<<grid, 64 * nw, 0, s>>>(a)) : (w4_matvec_kernel<T, G, R, 1><<<grid, 64 * nw, 0, s>>>(a)))
+    if (a.group % 128 == 0) W4_RUN(4); else if (a.group % 64 == 0) W4_RUN(2); else W4_RUN(1);
+#undef W4_RUN
+}
+
 int w4_check(int dtype, long K, long N, int group, const char* what) {
     if (!op_bytes(dtype)) return set_err(DPDF_E_INVALID, "%s: unsupported dtype %d", what, dtype);
     if (K < 1 || N < 1) return set_err(DPDF_E_INVALID, "%s: empty layer %ld x %ld", what, N, K);
@@ -182,9 +193,8 @@ extern "C" int dpdf_w4_matvec(int device, const dpdf_w4_matvec_args* args, void*
     OpDevice dev(device);
     HIP_TRY(dev.err);
     W4Args a{x.x, x.x_stride, x.codes, x.codes_pitch, x.scales, x.scales_stride, x.zeros, x.zeros_pitch, x.bias, x.out, x.out_stride, x.rows, x.in_dim, x.out_dim, x.group};
-    if ((x.rows + 7L) / 8 > 65535) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
-    const dim3 grid((unsigned)((x.out_dim + 3L) / 4), (unsigned)((x.rows + 7L) / 8));
-    gd_types(x.dtype, x.scale_dtype, [&](auto t, auto g) { w4_matvec_any_kernel<decltype(t), decltype(g)><<<grid, 256, 0, (hipStream_t)stream>>>(a); });
+    if ((x.rows + 15L) / 16 > 65535) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
+    gd_types(x.dtype, x.scale_dtype, [&](auto t, auto g) { w4_launch<decltype(t), decltype(g)>(a, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());
     return DPDF_OK;
 }
