@@ -4,6 +4,7 @@
 // (gated_delta_clip_kernel).  Value head h reads key head h / (Hv / Hk).
 #pragma once
 #include "common.h"
+#include "gru_limb.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -17,6 +18,8 @@ struct GatedDeltaArgs {
     long qs[3], ks[3], vs[3], gs[3], bs[3], os[3];      // strides in elements: batch, frame, head
     int T, Hk, Hv, Dk, Dv;
     int strips;                       // workgroups (clip) or waves (step) per head
+    int gate;                         // type of g and beta: 0 fp32, 1 fp16, 2 bf16
+    int whole;                        // clips: k and q can be read in pieces of eight values
     float scale;
 };
 
@@ -31,6 +34,9 @@ template <> __device__ __forceinline__ void gd_store<float>(void* p, long i, flo
 template <> __device__ __forceinline__ void gd_store<__half>(void* p, long i, float v) { ((__half*)p)[i] = __float2half(v); }
 template <> __device__ __forceinline__ void gd_store<__hip_bfloat16>(void* p, long i, float v) { ((__bf16*)p)[i] = (__bf16)v; }
 
+__device__ __forceinline__ float gd_gate(const void* p, long i, int type) {
+    return type == 0 ? gd_load<float>(p, i) : type == 1 ? gd_load<__half>(p, i) : gd_load<__hip_bfloat16>(p, i);
+}
 __device__ __forceinline__ bool gd_finite(float v) { return (__builtin_bit_cast(unsigned, v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float gd_nan() { return __builtin_bit_cast(float, 0x7fc00000u); }
 
@@ -40,7 +46,7 @@ __device__ __forceinline__ float gd_nan() { return __builtin_bit_cast(float, 0x7
 // sums over the OLD state, so that one butterfly over the eight row groups serves them, and no wave waits for another.
 // Bound: HBM, the state read once and written once.
 // ---------------------------------------------------------------------------------------------------------------------------------------
-template <typename T, typename G, int DKP, bool VEC>
+template <typename T, int DKP, bool WHOLE>
 __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) {
     constexpr int R = DKP / 8;
     const int lane = threadIdx.x, cl = lane & 7, rg = lane >> 3;
@@ -55,13 +61,12 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
     for (int j = 0; j < R; ++j) {
         const int r = r0 + j;
         const float* p = a.state_in + sbase + (long)r * a.Dv + c0;
-        if (VEC) {
-            const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-            const float4 s = a.state_in && r < a.Dk && c0 < a.Dv ? *(const float4*)p : z;
+        if constexpr (WHOLE) {
+            const float4 s = *(const float4*)p;
             S[j][0] = s.x; S[j][1] = s.y; S[j][2] = s.z; S[j][3] = s.w;
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][i] = a.state_in && r < a.Dk && c0 + i < a.Dv ? p[i] : 0.f;
+            for (int i = 0; i < 4; ++i) S[j][i] = r < a.Dk && c0 + i < a.Dv ? p[i] : 0.f;
         }
     }
     const long qb = (long)b * a.qs[0] + (long)hk * a.qs[2], kb = (long)b * a.ks[0] + (long)hk * a.ks[2];
@@ -71,13 +76,13 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
         float kr[R], qr[R], v[4];
 #pragma unroll
         for (int j = 0; j < R; ++j) {
-            const bool in = r0 + j < a.Dk;
+            const bool in = WHOLE || r0 + j < a.Dk;
             kr[j] = in ? gd_load<T>(a.k, kb + t * a.ks[1] + r0 + j) : 0.f;
             qr[j] = in ? gd_load<T>(a.q, qb + t * a.qs[1] + r0 + j) : 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = c0 + i < a.Dv ? gd_load<T>(a.v, vb + t * a.vs[1] + i) : 0.f;
-        const float alpha = __expf(gd_load<G>(a.g, gb + t * a.gs[1])), beta = gd_load<G>(a.beta, bb + t * a.bs[1]);
+        for (int i = 0; i < 4; ++i) v[i] = WHOLE || c0 + i < a.Dv ? gd_load<T>(a.v, vb + t * a.vs[1] + i) : 0.f;
+        const float alpha = __expf(gd_gate(a.g, gb + t * a.gs[1], a.gate)), beta = gd_gate(a.beta, bb + t * a.bs[1], a.gate);
         float sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f}, qk = 0.f;
 #pragma unroll
         for (int j = 0; j < R; ++j) {
@@ -105,55 +110,170 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
         if (rg == 0)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (c0 + i < a.Dv) gd_store<T>(a.out, ob + t * a.os[1] + i, a.scale * __builtin_fmaf(qk, e[i], sq[i]));
+                if (WHOLE || c0 + i < a.Dv) gd_store<T>(a.out, ob + t * a.os[1] + i, a.scale * __builtin_fmaf(qk, e[i], sq[i]));
     }
 #pragma unroll
     for (int j = 0; j < R; ++j) {
         const int r = r0 + j;
         float* p = a.state_out + sbase + (long)r * a.Dv + c0;
-        if (r >= a.Dk) continue;
-        if (VEC) {
-            if (c0 < a.Dv) *(float4*)p = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
-        } else {
+        if constexpr (WHOLE) *(float4*)p = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
+        else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (c0 + i < a.Dv) p[i] = S[j][i];
+                if (r < a.Dk && c0 + i < a.Dv) p[i] = S[j][i];
         }
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------
-// Clips: chunks of 64 frames.  With gamma = the running sum of g inside the chunk, d_ij = exp(gamma_i - gamma_j) and S the state before it,
+// Clips: chunks of C frames.  With gamma = the running sum of g inside the chunk, d_ij = exp(gamma_i - gamma_j) and S the state before it,
 //     A_ij = beta_i d_ij k_i.k_j (j < i),   (I + A) u = beta (v - exp(gamma) (K S)),
-//     O = scale exp(gamma) (Q S) + P u,   P_ij = scale d_ij q_i.k_j (j <= i),   S <- exp(gamma_63) S + K^T (exp(gamma_63 - gamma) u):
-// matrix products, and 16 dependent steps for the inverses of the four 16 x 16 diagonal blocks of I + A where the definition has 64.
-// A workgroup is one head and up to 64 columns: wave w owns 16 columns of S, u and O in the matrix units' result layout (row 4 q + i, column
-// n), in which a result IS the next product's right operand -- K slot 4 q + i of a block is its row 4 q + i -- so that K S -> u -> P u, K^T u
-// chain in registers, and the waves meet only over the chunk's K, Q, A and P in LDS.
+//     O = scale exp(gamma) (Q S) + P u,   P_ij = scale d_ij q_i.k_j (j <= i),   S <- exp(gamma_C) S + K^T (exp(gamma_C - gamma) u):
+// matrix products, and 16 dependent steps for the inverses of the 16 x 16 diagonal blocks of I + A where the definition has C.
+//
+// A workgroup is one head and 16 NW columns: wave w owns 16 columns of S, u and O in the matrix units' result layout (row 4 q + i, column n),
+// in which a result IS the next product's right operand -- K slot 8 q + 4 h + i of two 16-row blocks is row 4 q + i of block h -- so that
+// K S -> u -> P u, K^T u chain in registers, and the waves meet only over the chunk's K, Q, A and P in LDS, which are laid out in that order.
+//
+// Every fp32 operand goes in as bf16 limbs (split3 of gru_limb.h: exact), products of limbs whose indices add up to more than 2 (2^-24 of the
+// term) left out; bf16 values of k and q are one limb, fp16 two, fp32 three.  What only reaches the outputs of a 16-bit type (Q S, P u) takes two
+// limbs of either side, 2^-16 of a term against the 2^-8 and 2^-11 of the result's rounding; the state's path takes all.
+//
 // gamma and its differences are 64-bit: they are small differences of long sums.  A non-finite k, g or beta makes its head's outputs from its
-// frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all 64
+// frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all
 // frames of the chunk, so that such values are taken out of the operands first).
 // ---------------------------------------------------------------------------------------------------------------------------------------
-constexpr int GD_C = 64;
+template <typename T> struct GdIn;
+template <> struct GdIn<__hip_bfloat16> { enum { L = 1 }; };
+template <> struct GdIn<__half> { enum { L = 2 }; };
+template <> struct GdIn<float> { enum { L = 3 }; };
 
-template <typename T, typename G, int DKP>
-__global__ __launch_bounds__(256) void gated_delta_clip_kernel(GatedDeltaArgs a) {
-    constexpr int NB = DKP / 16, LD = DKP + 4, LA = GD_C + 4;
-    __shared__ __attribute__((aligned(16))) float Ks[GD_C][LD], Qs[GD_C][LD], As[GD_C][LA], Ps[GD_C][LA], Ti[4][16][20];
-    __shared__ double gam[GD_C];
-    __shared__ float eg[GD_C], ee[GD_C], bt[GD_C];
-    __shared__ int kbad;
-    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = lane & 15, q = lane >> 4;
+// the running sum over a wave's lanes
+__device__ __forceinline__ double gd_scan(double v) {
+#define GD_STEP_(ctrl, rows) { \
+        const unsigned long b = __builtin_bit_cast(unsigned long, v); \
+        const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, ctrl, rows, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), ctrl, rows, 0xf, false); \
+        v += __builtin_bit_cast(double, (unsigned long)hi << 32 | lo); }
+    GD_STEP_(0x111, 0xf) GD_STEP_(0x112, 0xf) GD_STEP_(0x114, 0xf) GD_STEP_(0x118, 0xf)      // row_shr 1, 2, 4, 8: inside 16 lanes
+    GD_STEP_(0x142, 0xa) GD_STEP_(0x143, 0xc)                                                // lane 15's sum to the next row, lane 31's to the upper half
+#undef GD_STEP_
+    return v;
+}
+// What a chunk reads and writes goes through buffer descriptors that end with its last frame: behind that, and at GD_OUT, loads give 0 and stores
+// do nothing, so that there is no branch around a load (behind one the compiler cannot count the loads in flight and waits for them), no
+// clamp and 32 bits of address.
+constexpr unsigned GD_OUT = 0x80000000u;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t gd_buffer(const void* base, long first, long count, int elem) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + first * elem), 0, (int)(count * elem), 0x00027000);
+}
+template <typename T> struct GdRow { T v[8]; };
+typedef unsigned gd_u4 __attribute__((ext_vector_type(4)));
+// eight values of a row, at `off` (whole: in one piece), the first `left` of them
+template <typename T> __device__ __forceinline__ GdRow<T> gd_row(__amdgpu_buffer_rsrc_t r, unsigned off, int left, bool whole) {
+    GdRow<T> x;
+    if (whole) {
+        const unsigned o = left > 0 ? off : GD_OUT;
+        gd_u4 v[sizeof(T) / 2];
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(T) / 2; ++e) v[e] = __builtin_amdgcn_raw_buffer_load_b128(r, o + 16 * e, 0, 0);
+        __builtin_memcpy(&x, v, sizeof(x));
+    } else
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const unsigned o = e < left ? off + e * (unsigned)sizeof(T) : GD_OUT;
+            if constexpr (sizeof(T) == 2) { const unsigned short v = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0); __builtin_memcpy(&x.v[e], &v, 2); }
+            else { const unsigned v = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0); __builtin_memcpy(&x.v[e], &v, 4); }
+        }
+    return x;
+}
+template <typename T> __device__ __forceinline__ unsigned gd_get(__amdgpu_buffer_rsrc_t r, unsigned off) {
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    else return __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+}
+template <typename T> __device__ __forceinline__ float gd_value(unsigned raw) {
+    if constexpr (__is_same(T, __hip_bfloat16)) return __builtin_bit_cast(float, raw << 16);
+    else if constexpr (__is_same(T, __half)) return (float)__builtin_bit_cast(_Float16, (unsigned short)raw);
+    else return __builtin_bit_cast(float, raw);
+}
+template <typename T> __device__ __forceinline__ void gd_put(__amdgpu_buffer_rsrc_t r, unsigned off, float v) {
+    if constexpr (__is_same(T, __hip_bfloat16)) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), r, off, 0, 0);
+    else if constexpr (__is_same(T, __half)) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (_Float16)v), r, off, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, off, 0, 0);
+}
+// the row's limbs, 8 x 16 bit each; true where a value is not finite
+template <typename T> __device__ __forceinline__ bool gd_limbs(const GdRow<T>& r, uint4 (&f)[GdIn<T>::L]) {
+    if constexpr (GdIn<T>::L == 1) {
+        f[0] = __builtin_bit_cast(uint4, r);
+        // an exponent of all ones carries into the sign's place
+        const unsigned t = ((f[0].x & 0x7f807f80u) + 0x00800080u) | ((f[0].y & 0x7f807f80u) + 0x00800080u) | ((f[0].z & 0x7f807f80u) + 0x00800080u) | ((f[0].w & 0x7f807f80u) + 0x00800080u);
+        return t & 0x80008000u;
+    } else {
+        float x[8], t = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { x[e] = gd_load<T>(r.v, e); t = __builtin_fmaf(x[e], 0.f, t); }
+        uint2 l[2][3];
+        split3(make_float4(x[0], x[1], x[2], x[3]), l[0][0], l[0][1], l[0][2]);
+        split3(make_float4(x[4], x[5], x[6], x[7]), l[1][0], l[1][1], l[1][2]);
+#pragma unroll
+        for (int e = 0; e < GdIn<T>::L; ++e) f[e] = make_uint4(l[0][e].x, l[0][e].y, l[1][e].x, l[1][e].y);
+        return !(t == 0.f);
+    }
+}
+// the limbs of four values into the lower or upper half of a fragment of each
+template <int N> __device__ __forceinline__ void gd_split(const f32x4& v, uint4 (&f)[N], int half) {
+    float r0 = v[0], r1 = v[1], r2 = v[2], r3 = v[3];
+#pragma unroll
+    for (int l = 0; l < N; ++l) {
+        const unsigned p = pk_bf16(r0, r1), s = pk_bf16(r2, r3);
+        if (half) { f[l].z = p; f[l].w = s; } else { f[l].x = p; f[l].y = s; }
+        if (l + 1 < N) { r0 -= bf_lo(p); r1 -= bf_hi(p); r2 -= bf_lo(s); r3 -= bf_hi(s); }
+    }
+}
+// acc + a b over 32 slots, NA limbs by NB limbs, pairs up to TOP
+template <int TOP, int NA, int NB> __device__ __forceinline__ f32x4 gd_mul(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 acc) {
+#pragma unroll
+    for (int o = TOP; o >= 0; --o)
+#pragma unroll
+        for (int l = 0; l < NA; ++l)
+            if (o - l >= 0 && o - l < NB) acc = mfma_bf16(a[l], b[o - l], acc);
+    return acc;
+}
+// the same over 16 slots, those of the lower halves: two limbs of a side share a fragment
+__device__ __forceinline__ uint4 gd_two(const uint4& x, const uint4& y) { return make_uint4(x.x, x.y, y.x, y.y); }
+template <int N> __device__ __forceinline__ f32x4 gd_mul16(const uint2 (&a)[N], const uint4* b, f32x4 acc) {
+    const uint4 a01 = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
+    if constexpr (N == 3) acc = mfma_bf16(make_uint4(a[0].x, a[0].y, a[2].x, a[2].y), gd_two(b[2], b[0]), acc);
+    acc = mfma_bf16(a01, gd_two(b[1], b[1]), acc);
+    return mfma_bf16(a01, gd_two(b[0], b[0]), acc);
+}
+
+template <typename T, int DKP, int NW, int C>
+__global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDeltaArgs a) {
+    constexpr int L = GdIn<T>::L, NB = DKP / 16, NC = DKP / 32, CB = C / 16, CC = C / 32, LDK = DKP + 8, LDT = C + 8, E = sizeof(T);
+    constexpr int BLOCKS = CB * (CB + 1) / 2;
+    constexpr bool WIDE = E == 4;                          // outputs of 32 bits
+    constexpr int PL = WIDE ? 3 : 2, ITEMS = (C / 2 * (DKP / 8) + 64 * NW - 1) / (64 * NW);
+    // blocks of A below the diagonal and of P on and below it, two neighbours of a row to a fragment: row bi of A starts at bi^2 / 4, of P at (bi + 1)^2 / 4
+    constexpr int ASLOTS = CB * CB / 4, PSLOTS = (CB + 1) * (CB + 1) / 4;
+    __shared__ __attribute__((aligned(16))) unsigned short Kr[L][C][LDK], Qr[L][C][LDK], Kt[L][DKP][LDT];
+    __shared__ __attribute__((aligned(16))) uint2 Af[ASLOTS][3][64][2], Pf[PSLOTS][PL][64][2];
+    __shared__ __attribute__((aligned(16))) float Ad[CB][16][20];
+    __shared__ __attribute__((aligned(16))) float2 gam[C];
+    __shared__ __attribute__((aligned(16))) float eg[C], ee[C], bt[C];
+    __shared__ int kbad[2];
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
     const long head = blockIdx.x / a.strips;
     const int b = (int)(head / a.Hv), h = (int)(head - (long)b * a.Hv), hk = h / (a.Hv / a.Hk);
-    const int col = 64 * (int)(blockIdx.x - head * a.strips) + 16 * w + n;
+    const int c0w = 16 * NW * (int)(blockIdx.x - head * a.strips) + 16 * w, col = c0w + n;
     const bool cin = col < a.Dv;
     int len = a.lengths ? a.lengths[b] : a.T;
     len = len < 0 ? 0 : len > a.T ? a.T : len;
     const long qb = (long)b * a.qs[0] + (long)hk * a.qs[2], kb = (long)b * a.ks[0] + (long)hk * a.ks[2];
-    const long vb = (long)b * a.vs[0] + (long)h * a.vs[2] + col, ob = (long)b * a.os[0] + (long)h * a.os[2] + col;
+    const long vb = (long)b * a.vs[0] + (long)h * a.vs[2], ob = (long)b * a.os[0] + (long)h * a.os[2];
     const long gb = (long)b * a.gs[0] + (long)h * a.gs[2], bb = (long)b * a.bs[0] + (long)h * a.bs[2];
     const long sb = head * a.Dk * a.Dv + col;
+    const unsigned vstep = (unsigned)a.vs[1] * E, ostep = (unsigned)a.os[1] * E;
+    const unsigned voff = cin ? 4 * q * vstep + col * E : GD_OUT, ooff = cin ? 4 * q * ostep + col * E : GD_OUT;
     f32x4 S[NB];
 #pragma unroll
     for (int c = 0; c < NB; ++c)
@@ -162,119 +282,252 @@ __global__ __launch_bounds__(256) void gated_delta_clip_kernel(GatedDeltaArgs a)
             const int r = 16 * c + 4 * q + i;
             S[c][i] = a.state_in && cin && r < a.Dk ? a.state_in[sb + (long)r * a.Dv] : 0.f;
         }
-    for (int t0 = 0; t0 < len; t0 += GD_C) {
-        const int m = len - t0 < GD_C ? len - t0 : GD_C;
-        __syncthreads();
-        if (tid == 0) kbad = GD_C;
-        __syncthreads();
-        for (int e = tid; e < GD_C * DKP; e += 256) {
-            const int r = e / DKP, c = e - r * DKP;
-            const bool in = r < m && c < a.Dk;
-            float kv = in ? gd_load<T>(a.k, kb + (long)(t0 + r) * a.ks[1] + c) : 0.f;
-            if (!gd_finite(kv)) { atomicMin(&kbad, r); kv = 0.f; }
-            Ks[r][c] = kv;
-            Qs[r][c] = in ? gd_load<T>(a.q, qb + (long)(t0 + r) * a.qs[1] + c) : 0.f;
-        }
-        if (tid < GD_C) {
-            float gv = tid < m ? gd_load<G>(a.g, gb + (long)(t0 + tid) * a.gs[1]) : 0.f;
-            float bv = tid < m ? gd_load<G>(a.beta, bb + (long)(t0 + tid) * a.bs[1]) : 0.f;
-            if (!(gv < __builtin_inff()) || !gd_finite(bv)) { atomicMin(&kbad, tid); gv = 0.f; bv = 0.f; }
-            double s = (gv < -128.f ? -128.0 : (double)gv) * 1.4426950408889634;      // in powers of two; exp(-128) is 0 in fp32 already: -inf,
-                                                                                      // a reset, comes without inf - inf
+
+    // a chunk on its way: two rows of eight k and q per item, this lane's v, the gates of frame `lane`
+    GdRow<T> nk[ITEMS][2], nq[ITEMS][2];
+    unsigned nv[CB][4];
+    float ng = 0.f, nbt = 0.f;
+    const bool whole = a.whole;
+    auto fetch = [&](int t0) {
+        const int m = len - t0 < C ? len - t0 : C;
+        const auto rk = gd_buffer(a.k, kb + (long)t0 * a.ks[1], (m - 1) * a.ks[1] + a.Dk, E), rq = gd_buffer(a.q, qb + (long)t0 * a.qs[1], (m - 1) * a.qs[1] + a.Dk, E);
+        const auto rv = gd_buffer(a.v, vb + (long)t0 * a.vs[1], (m - 1) * a.vs[1] + a.Dv, E);
 #pragma unroll
-            for (int o = 1; o < 64; o <<= 1) { const double u = __shfl_up(s, o); if (tid >= o) s += u; }
-            gam[tid] = s; bt[tid] = bv;
-            eg[tid] = __builtin_amdgcn_exp2f((float)s);
-            ee[tid] = __builtin_amdgcn_exp2f((float)(__shfl(s, 63) - s));
-        }
-        __syncthreads();
-        // A and P, ten 16 x 16 blocks on and below the diagonal of each
-        for (int e = w; e < 20; e += 4) {
-            const bool isq = e >= 10;
-            int f = isq ? e - 10 : e, bi = 0;
-            while (f > bi) { f -= bi + 1; ++bi; }
-            const int bj = f;
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            for (int c = 0; c < NB; ++c) {
-                const float4 x = *(const float4*)(isq ? &Qs[16 * bi + n][16 * c + 4 * q] : &Ks[16 * bi + n][16 * c + 4 * q]);
-                const float4 y = *(const float4*)&Ks[16 * bj + n][16 * c + 4 * q];
-                acc = mfma16(x.x, y.x, acc); acc = mfma16(x.y, y.y, acc); acc = mfma16(x.z, y.z, acc); acc = mfma16(x.w, y.w, acc);
+        for (int it = 0; it < ITEMS; ++it) {
+            const int e = tid + 64 * NW * it, j = e % (DKP / 8), p = e / (DKP / 8);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                nk[it][x] = gd_row<T>(rk, (2 * p + x) * (unsigned)a.ks[1] * E + 8 * j * E, a.Dk - 8 * j, whole);
+                nq[it][x] = gd_row<T>(rq, (2 * p + x) * (unsigned)a.qs[1] * E + 8 * j * E, a.Dk - 8 * j, whole);
             }
+        }
+#pragma unroll
+        for (int bl = 0; bl < CB; ++bl)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) nv[bl][i] = gd_get<T>(rv, voff + (16 * bl + i) * vstep);
+        if (w == 0) {
+            const int r = t0 + (lane < m ? lane : m - 1);
+            ng = gd_gate(a.g, gb + (long)r * a.gs[1], a.gate);
+            nbt = gd_gate(a.beta, bb + (long)r * a.bs[1], a.gate);
+        }
+    };
+    if (tid < 2) kbad[tid] = C;
+    if (len > 0) fetch(0);
+    for (int t0 = 0, par = 0; t0 < len; t0 += C, par ^= 1) {
+        const int m = len - t0 < C ? len - t0 : C;
+        __syncthreads();
+#pragma unroll
+        for (int it = 0; it < ITEMS; ++it) {
+            const int e = tid + 64 * NW * it, j = e % (DKP / 8), p = e / (DKP / 8);
+            if (p >= C / 2) break;
+            uint4 kl[2][L], ql[2][L];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if (gd_limbs<T>(nk[it][x], kl[x])) {
+                    atomicMin(&kbad[par], 2 * p + x);
+#pragma unroll
+                    for (int l = 0; l < L; ++l) kl[x][l] = make_uint4(0, 0, 0, 0);
+                }
+                gd_limbs<T>(nq[it][x], ql[x]);
+            }
+            const int c0 = 32 * (j >> 2) + 8 * (2 * j & 3) + 4 * (j >> 1 & 1);                    // slots of k 8 j .. 8 j + 3; the next four are 8 on
+            const int r0 = 2 * p, tc = 32 * (r0 >> 5) + 8 * (r0 >> 2 & 3) + 4 * (r0 >> 4 & 1) + (r0 & 3);
+#pragma unroll
+            for (int l = 0; l < L; ++l) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    *(uint2*)&Kr[l][r0 + x][c0] = make_uint2(kl[x][l].x, kl[x][l].y); *(uint2*)&Kr[l][r0 + x][c0 + 8] = make_uint2(kl[x][l].z, kl[x][l].w);
+                    *(uint2*)&Qr[l][r0 + x][c0] = make_uint2(ql[x][l].x, ql[x][l].y); *(uint2*)&Qr[l][r0 + x][c0 + 8] = make_uint2(ql[x][l].z, ql[x][l].w);
+                }
+                const unsigned u0[4] = {kl[0][l].x, kl[0][l].y, kl[0][l].z, kl[0][l].w}, u1[4] = {kl[1][l].x, kl[1][l].y, kl[1][l].z, kl[1][l].w};
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    *(unsigned*)&Kt[l][8 * j + 2 * d][tc] = __builtin_amdgcn_perm(u1[d], u0[d], 0x05040100u);
+                    *(unsigned*)&Kt[l][8 * j + 2 * d + 1][tc] = __builtin_amdgcn_perm(u1[d], u0[d], 0x07060302u);
+                }
+            }
+        }
+        if (w == 0) {
+            if (lane >= m) { ng = 0.f; nbt = 0.f; }
+            if (!(ng < __builtin_inff()) || !gd_finite(nbt)) { atomicMin(&kbad[par], lane); ng = 0.f; nbt = 0.f; }
+            // in powers of two; exp(-128) is 0 in fp32 already: -inf, a reset, comes without inf - inf
+            const double s = gd_scan((ng < -128.f ? -128.0 : (double)ng) * 1.4426950408889634);
+            const double last = __shfl(s, C - 1);
+            if (lane < C) {
+                const float hi = (float)s;
+                gam[lane] = make_float2(hi, (float)(s - (double)hi)); bt[lane] = nbt;
+                eg[lane] = __builtin_amdgcn_exp2f(hi);
+                ee[lane] = __builtin_amdgcn_exp2f((float)(last - s));
+            }
+        }
+        float v[CB][4], vsum = 0.f;
+#pragma unroll
+        for (int bl = 0; bl < CB; ++bl)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[bl][i] = gd_value<T>(nv[bl][i]); vsum = __builtin_fmaf(v[bl][i], 0.f, vsum); }
+        __syncthreads();
+        if (t0 + C < len) fetch(t0 + C);
+        if (tid == 0) kbad[par ^ 1] = C;
+        // A and P, the 16 x 16 blocks on and below the diagonal, as their transposes: a lane then holds what it will read, [row n][4 q ..]
+        for (int e = w; e < BLOCKS; e += NW) {
+            int bi = 0, bj = e;
+            while (bj > bi) { bj -= bi + 1; ++bi; }
+            f32x4 xa = {0.f, 0.f, 0.f, 0.f}, xp = xa;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                uint4 kj[L], ki[L], qi[L];
+#pragma unroll
+                for (int l = 0; l < L; ++l) {
+                    kj[l] = *(const uint4*)&Kr[l][16 * bj + n][32 * c + 8 * q];
+                    ki[l] = *(const uint4*)&Kr[l][16 * bi + n][32 * c + 8 * q];
+                    qi[l] = *(const uint4*)&Qr[l][16 * bi + n][32 * c + 8 * q];
+                }
+                xa = gd_mul<2>(kj, ki, xa);
+                xp = gd_mul<2>(kj, qi, xp);
+            }
+            const float2 gr = gam[16 * bi + n];
+            const float br = -bt[16 * bi + n];
+            const float4 g01 = *(const float4*)&gam[16 * bj + 4 * q], g23 = *(const float4*)&gam[16 * bj + 4 * q + 2];
+            const float gh[4] = {g01.x, g01.z, g23.x, g23.z}, gl[4] = {g01.y, g01.w, g23.y, g23.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int r = 16 * bi + 4 * q + i, s = 16 * bj + n;
-                const float d = s <= r ? __builtin_amdgcn_exp2f((float)(gam[r] - gam[s])) : 0.f;
-                if (isq) Ps[r][s] = s <= r ? a.scale * d * acc[i] : 0.f;
-                else As[r][s] = s < r ? bt[r] * d * acc[i] : 0.f;
+                const float d = __builtin_amdgcn_exp2f((gr.x - gh[i]) + (gr.y - gl[i]));
+                xa[i] *= br * d;
+                xp[i] *= a.scale * d;
             }
+            if (bi == bj) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (4 * q + i >= n) xa[i] = 0.f;
+                    if (4 * q + i > n) xp[i] = 0.f;
+                }
+                *(float4*)&Ad[bi][n][4 * q] = make_float4(xa[0], xa[1], xa[2], xa[3]);
+            } else {
+                uint4 f[3];
+                gd_split(xa, f, 0);
+#pragma unroll
+                for (int l = 0; l < 3; ++l) Af[bi * bi / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
+            }
+            uint4 f[PL];
+            gd_split(xp, f, 0);
+#pragma unroll
+            for (int l = 0; l < PL; ++l) Pf[(bi + 1) * (bi + 1) / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
         }
         __syncthreads();
-        if (lane < 16) {          // inverse of diagonal block w of I + A: lane = column, forward substitution
+        // inverses of the diagonal blocks of I + A: lane = column, forward substitution, in place
+        for (int bl = w; bl < CB; bl += NW) {
             float t[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                float s = i == lane ? 1.f : 0.f;
+                float s = i == n ? 1.f : 0.f;
 #pragma unroll
-                for (int j = 0; j < i; ++j) s = __builtin_fmaf(-As[16 * w + i][16 * w + j], t[j], s);
+                for (int j = 0; j < i; ++j) s = __builtin_fmaf(Ad[bl][i][j], t[j], s);
                 t[i] = s;
-                Ti[w][i][lane] = s;
+            }
+            if (lane < 16)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) Ad[bl][i][lane] = t[i];
+        }
+        // x = K S, y = Q S
+        f32x4 x[CB], y[CB];
+        {
+            uint4 sl[NC][3];
+#pragma unroll
+            for (int c = 0; c < NB; ++c) gd_split(S[c], sl[c / 2], c & 1);
+#pragma unroll
+            for (int bl = 0; bl < CB; ++bl) {
+                x[bl] = (f32x4){0.f, 0.f, 0.f, 0.f}; y[bl] = x[bl];
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    uint4 kf[L], qf[L];
+#pragma unroll
+                    for (int l = 0; l < L; ++l) { kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q]; qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q]; }
+                    x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
+                    y[bl] = gd_mul<WIDE ? 2 : 1>(qf, sl[c], y[bl]);
+                }
             }
         }
         __syncthreads();
-        f32x4 u[4], o[4];
-        int bad = kbad;
+        int bad = kbad[par];
+        if (__any(!(vsum == 0.f) || bad < C)) {
 #pragma unroll
-        for (int bl = 0; bl < 4; ++bl) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+            for (int bl = 0; bl < CB; ++bl)
 #pragma unroll
-            for (int c = 0; c < NB; ++c) {
-                const float4 kk = *(const float4*)&Ks[16 * bl + n][16 * c + 4 * q], qq = *(const float4*)&Qs[16 * bl + n][16 * c + 4 * q];
-                x = mfma16(kk.x, S[c][0], x); x = mfma16(kk.y, S[c][1], x); x = mfma16(kk.z, S[c][2], x); x = mfma16(kk.w, S[c][3], x);
-                y = mfma16(qq.x, S[c][0], y); y = mfma16(qq.y, S[c][1], y); y = mfma16(qq.z, S[c][2], y); y = mfma16(qq.w, S[c][3], y);
-            }
-            f32x4 z = {0.f, 0.f, 0.f, 0.f};
-            for (int c = 0; c < bl; ++c) {
-                const float4 aa = *(const float4*)&As[16 * bl + n][16 * c + 4 * q];
-                z = mfma16(aa.x, u[c][0], z); z = mfma16(aa.y, u[c][1], z); z = mfma16(aa.z, u[c][2], z); z = mfma16(aa.w, u[c][3], z);
-            }
-            f32x4 rhs;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 16 * bl + 4 * q + i;
-                float v = cin && r < m ? gd_load<T>(a.v, vb + (long)(t0 + r) * a.vs[1]) : 0.f;
-                if (!gd_finite(v)) { bad = r < bad ? r : bad; v = 0.f; }
-                rhs[i] = __builtin_fmaf(bt[r], __builtin_fmaf(-eg[r], x[i], v), -z[i]);
-                o[bl][i] = a.scale * eg[r] * y[i];
-            }
-            const float4 ti = *(const float4*)&Ti[bl][n][4 * q];
-            f32x4 uu = {0.f, 0.f, 0.f, 0.f};
-            uu = mfma16(ti.x, rhs[0], uu); uu = mfma16(ti.y, rhs[1], uu); uu = mfma16(ti.z, rhs[2], uu); uu = mfma16(ti.w, rhs[3], uu);
-            u[bl] = uu;
-            for (int c = 0; c <= bl; ++c) {
-                const float4 pp = *(const float4*)&Ps[16 * bl + n][16 * c + 4 * q];
-                o[bl] = mfma16(pp.x, u[c][0], o[bl]); o[bl] = mfma16(pp.y, u[c][1], o[bl]); o[bl] = mfma16(pp.z, u[c][2], o[bl]); o[bl] = mfma16(pp.w, u[c][3], o[bl]);
-            }
+                for (int i = 0; i < 4; ++i)
+                    if (!gd_finite(v[bl][i])) { const int r = 16 * bl + 4 * q + i; bad = r < bad ? r : bad; v[bl][i] = 0.f; }
+            { const int z = __shfl_xor(bad, 16); bad = z < bad ? z : bad; }
+            { const int z = __shfl_xor(bad, 32); bad = z < bad ? z : bad; }
         }
-        { const int x = __shfl_xor(bad, 16); bad = x < bad ? x : bad; }
-        { const int x = __shfl_xor(bad, 32); bad = x < bad ? x : bad; }
-        const float end = eg[GD_C - 1];
+        const auto ro = gd_buffer(a.out, ob + (long)t0 * a.os[1], (m - 1) * a.os[1] + a.Dv, E);
+        uint4 ul[CC][3], wl[CC][3];
+        f32x4 o[CB];
 #pragma unroll
-        for (int bl = 0; bl < 4; ++bl)
+        for (int bl = 0; bl < CB; ++bl) {
+            const float4 be = *(const float4*)&bt[16 * bl + 4 * q], e4 = *(const float4*)&eg[16 * bl + 4 * q], f4 = *(const float4*)&ee[16 * bl + 4 * q];
+            f32x4 z;
+            z[0] = be.x * __builtin_fmaf(-e4.x, x[bl][0], v[bl][0]); z[1] = be.y * __builtin_fmaf(-e4.y, x[bl][1], v[bl][1]);
+            z[2] = be.z * __builtin_fmaf(-e4.z, x[bl][2], v[bl][2]); z[3] = be.w * __builtin_fmaf(-e4.w, x[bl][3], v[bl][3]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 16 * bl + 4 * q + i;
-                if (cin && r < m) gd_store<T>(a.out, ob + (long)(t0 + r) * a.os[1], r >= bad ? gd_nan() : o[bl][i]);
-                u[bl][i] *= ee[r];
+            for (int c = 0; c < bl / 2; ++c) {
+                uint4 f[3];
+#pragma unroll
+                for (int l = 0; l < 3; ++l) f[l] = *(const uint4*)Af[bl * bl / 4 + c][l][lane];
+                z = gd_mul<2>(f, ul[c], z);
             }
+            if (bl & 1) {
+                uint2 f[3];
+#pragma unroll
+                for (int l = 0; l < 3; ++l) f[l] = Af[bl * bl / 4 + bl / 2][l][lane][0];
+                z = gd_mul16(f, ul[bl / 2], z);
+            }
+            const float4 t = *(const float4*)&Ad[bl][n][4 * q];
+            f32x4 u = {0.f, 0.f, 0.f, 0.f};
+            u = mfma16(t.x, z[0], u); u = mfma16(t.y, z[1], u); u = mfma16(t.z, z[2], u); u = mfma16(t.w, z[3], u);
+            gd_split(u, ul[bl / 2], bl & 1);
+            o[bl][0] = a.scale * e4.x * y[bl][0]; o[bl][1] = a.scale * e4.y * y[bl][1]; o[bl][2] = a.scale * e4.z * y[bl][2]; o[bl][3] = a.scale * e4.w * y[bl][3];
+#pragma unroll
+            for (int c = 0; c < (bl + 1) / 2; ++c) {
+                uint4 f[PL];
+#pragma unroll
+                for (int l = 0; l < PL; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
+                o[bl] = gd_mul<PL - 1>(f, ul[c], o[bl]);
+            }
+            if (!(bl & 1)) {
+                uint2 f[PL];
+#pragma unroll
+                for (int l = 0; l < PL; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
+                o[bl] = gd_mul16(f, ul[bl / 2], o[bl]);
+            }
+            u[0] *= f4.x; u[1] *= f4.y; u[2] *= f4.z; u[3] *= f4.w;
+            gd_split(u, wl[bl / 2], bl & 1);
+        }
+        const float end = eg[C - 1];
 #pragma unroll
         for (int c = 0; c < NB; ++c) {
             S[c] *= end;
 #pragma unroll
-            for (int bl = 0; bl < 4; ++bl)
+            for (int k2 = 0; k2 < CC; ++k2) {
+                uint4 f[L];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) S[c] = mfma16(Ks[16 * bl + 4 * q + i][16 * c + n], u[bl][i], S[c]);
-            if (bad < GD_C) { const float x = gd_nan(); S[c] = (f32x4){x, x, x, x}; }
+                for (int l = 0; l < L; ++l) f[l] = *(const uint4*)&Kt[l][16 * c + n][32 * k2 + 8 * q];
+                S[c] = gd_mul<2>(f, wl[k2], S[c]);
+            }
         }
+        if (__any(bad < C)) {
+            const float z = gd_nan();
+            if (bad < C)
+#pragma unroll
+                for (int c = 0; c < NB; ++c) S[c] = (f32x4){z, z, z, z};
+#pragma unroll
+            for (int bl = 0; bl < CB; ++bl)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (16 * bl + 4 * q + i >= bad) o[bl][i] = z;
+        }
+#pragma unroll
+        for (int bl = 0; bl < CB; ++bl)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gd_put<T>(ro, ooff + (16 * bl + i) * ostep, o[bl][i]);
     }
     if (a.state_out && cin)
 #pragma unroll

@@ -1,6 +1,9 @@
 // host_operators.h -- C entry points of the stand-alone operators (gated_delta.h, w4_matvec.h): device pointers, the caller's stream, nothing
 // allocated, nothing waited for, so that every call can be captured into a graph.  Arguments are checked before anything is launched.
 
+#ifndef GD_CHUNK
+#define GD_CHUNK 64
+#endif
 namespace {
 struct OpDevice {                                 // the call's device for as long as it runs, the caller's afterwards
     int before = -1; hipError_t err;
@@ -75,22 +78,27 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
         a.qs[i] = x.q_stride[i]; a.ks[i] = x.k_stride[i]; a.vs[i] = x.v_stride[i];
         a.gs[i] = x.g_stride[i]; a.bs[i] = x.beta_stride[i]; a.os[i] = x.out_stride[i];
     }
-    a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale;
+    a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale; a.gate = x.gate_dtype;
     return DPDF_OK;
 }
 
-template <typename T, typename G>
-void gd_launch_step(const GatedDeltaArgs& a, unsigned grid, bool vec, hipStream_t s) {
-#define GD_STEP(D) (vec ? (gated_delta_step_kernel<T, G, D, true><<<grid, 64, 0, s>>>(a)) : (gated_delta_step_kernel<T, G, D, false><<<grid, 64, 0, s>>>(a)))
+template <typename T>
+void gd_launch_step(const GatedDeltaArgs& a, unsigned grid, bool even, hipStream_t s) {
+#define GD_STEP(D) (even && a.Dk == D ? (gated_delta_step_kernel<T, D, true><<<grid, 64, 0, s>>>(a)) : (gated_delta_step_kernel<T, D, false><<<grid, 64, 0, s>>>(a)))
     if (a.Dk <= 16) GD_STEP(16); else if (a.Dk <= 32) GD_STEP(32); else if (a.Dk <= 64) GD_STEP(64); else GD_STEP(128);
 #undef GD_STEP
 }
-template <typename T, typename G>
-void gd_launch_clip(const GatedDeltaArgs& a, unsigned grid, hipStream_t s) {
-    if (a.Dk <= 16) gated_delta_clip_kernel<T, G, 16><<<grid, 256, 0, s>>>(a);
-    else if (a.Dk <= 32) gated_delta_clip_kernel<T, G, 32><<<grid, 256, 0, s>>>(a);
-    else if (a.Dk <= 64) gated_delta_clip_kernel<T, G, 64><<<grid, 256, 0, s>>>(a);
-    else gated_delta_clip_kernel<T, G, 128><<<grid, 256, 0, s>>>(a);
+template <typename T, int NW>
+void gd_launch_clip(GatedDeltaArgs& a, long heads, hipStream_t s) {
+    a.strips = (a.Dv + 16 * NW - 1) / (16 * NW);
+    const unsigned grid = (unsigned)(heads * a.strips);
+    constexpr int C = sizeof(T) == 4 ? 32 : GD_CHUNK;
+    if (a.Dk <= 32) gated_delta_clip_kernel<T, 32, NW, C><<<grid, 64 * NW, 0, s>>>(a);
+    else if (a.Dk <= 64) gated_delta_clip_kernel<T, 64, NW, C><<<grid, 64 * NW, 0, s>>>(a);
+    else gated_delta_clip_kernel<T, 128, NW, C><<<grid, 64 * NW, 0, s>>>(a);
+}
+template <typename F> void gd_type(int dtype, F f) {
+    if (dtype == DPDF_F32) f(float()); else if (dtype == DPDF_F16) f(__half()); else f(__hip_bfloat16());
 }
 // calls f with the types of the values and of the gates
 template <typename F> void gd_types(int dtype, int gate, F f) {
@@ -122,11 +130,19 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
     GatedDeltaArgs a;
     if (int rc = gd_check(args, false, a)) return rc;
     if (!args->batch || (!args->frames && !args->state_out)) return DPDF_OK;
+    // a chunk's rows are addressed with 32 bits
+    const long most = (1L << 31) - 1, rows = args->frames < 1 ? 1 : args->frames < GD_CHUNK ? args->frames : GD_CHUNK, e = op_bytes(args->dtype);
+    for (const long* s : {args->q_stride, args->k_stride, args->v_stride, args->out_stride})
+        if (s[1] > (most - (long)(a.Dk > a.Dv ? a.Dk : a.Dv) * e) / (rows * e)) return set_err(DPDF_E_INVALID, "gated delta rule: a stride of %ld from frame to frame is too large", s[1]);
+    a.whole = a.Dk % 8 == 0;
+    for (const void* p : {a.q, a.k}) a.whole &= op_aligned(p, 4);
+    for (const long* s : {a.qs, a.ks}) for (int i = 0; i < 3; ++i) a.whole &= s[i] * e % 4 == 0;
     OpDevice dev(device);
     HIP_TRY(dev.err);
-    a.strips = (a.Dv + 63) / 64;
-    const unsigned grid = (unsigned)((long)args->batch * a.Hv * a.strips);
-    gd_types(args->dtype, args->gate_dtype, [&](auto t, auto g) { gd_launch_clip<decltype(t), decltype(g)>(a, grid, (hipStream_t)stream); });
+    gd_type(args->dtype, [&](auto t) {
+        if (a.Dv <= 64) gd_launch_clip<decltype(t), 4>(a, (long)args->batch * a.Hv, (hipStream_t)stream);
+        else gd_launch_clip<decltype(t), 8>(a, (long)args->batch * a.Hv, (hipStream_t)stream);
+    });
     HIP_TRY(hipGetLastError());
     return DPDF_OK;
 }
@@ -139,8 +155,8 @@ extern "C" int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* ar
     HIP_TRY(dev.err);
     a.strips = (a.Dv + 31) / 32;
     const unsigned grid = (unsigned)((long)args->batch * a.Hv * a.strips);
-    const bool vec = a.Dv % 4 == 0 && op_aligned(a.state_in, 16) && op_aligned(a.state_out, 16);
-    gd_types(args->dtype, args->gate_dtype, [&](auto t, auto g) { gd_launch_step<decltype(t), decltype(g)>(a, grid, vec, (hipStream_t)stream); });
+    const bool even = a.Dv % 32 == 0 && op_aligned(a.state_in, 16) && op_aligned(a.state_out, 16);
+    gd_type(args->dtype, [&](auto t) { gd_launch_step<decltype(t)>(a, grid, even, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());
     return DPDF_OK;
 }

@@ -126,7 +126,7 @@ def _c_gated(step=False, **change):
     (dict(q_stride=(-1, 1, 1)), "negative stride"), (dict(out_stride=(0, 32, 8)), "share"), (dict(out_stride=(96, 32, 7)), "share"), (dict(out_stride=(96, 24, 8)), "share"),
     (dict(out=0x3000000), "overlaps an input"), (dict(out=0x1000000 - 2), "overlaps an input"), (dict(out=0x7000000), "out overlaps"),
     (dict(state_out=0x7000004), "in part"), (dict(state_out=0x2000000), "overlaps an input"), (dict(active=0x9000000), "mask"),
-    (dict(batch=1 << 30), "too large"),
+    (dict(batch=1 << 30), "too large"), (dict(k=1 << 45, k_stride=(1 << 38, 1 << 30, 16)), "frame to frame"), (dict(out=1 << 45, out_stride=(1 << 40, 1 << 31, 8)), "frame to frame"),
 ])
 def test_gated_delta_refusals(change, word):
     rc, msg = _c_gated(**change)
@@ -143,6 +143,7 @@ def test_gated_delta_step_refusals_and_empty_calls():
     assert _c_gated(batch=0)[0] == 0 and _c_gated(step=True, batch=0)[0] == 0 and _c_gated(step=True, frames=0)[0] == 0
     assert _c_gated(frames=0, state_out=None)[0] == 0
     if backend.device_count() == 0:
+        assert _c_gated(frames=0)[0] == -2                                 # the states are still to be written
         assert _c_gated()[0] == -2 and _c_gated(step=True)[0] == -2        # no GPU: a failure, nothing computed elsewhere
 
 
