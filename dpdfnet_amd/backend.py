@@ -55,7 +55,7 @@ EXPORTED_SYMBOLS = (
     "dpdf_streams_prime_one", "dpdf_streams_is_primed", "dpdf_recovery_count", "dpdf_progress",
     "dpdf_enhance_batch_rows", "dpdf_streams_pool_config", "dpdf_streams_pool_tune", "dpdf_streams_slot_use", "dpdf_streams_submit_wait",
     "dpdf_streams_submit_many", "dpdf_streams_submit_block", "dpdf_streams_pool_stats", "dpdf_streams_pool_timing",
-    "dpdf_gated_delta", "dpdf_gated_delta_step", "dpdf_w4_quantize", "dpdf_w4_matvec",
+    "dpdf_gated_delta", "dpdf_gated_delta_workspace", "dpdf_gated_delta_step", "dpdf_w4_quantize", "dpdf_w4_matvec",
 )
 
 
@@ -233,7 +233,10 @@ def load_library() -> ctypes.CDLL:
         L.dpdf_resample_len.restype = ctypes.c_long
         L.dpdf_resample_len.argtypes = [ctypes.c_long, ctypes.c_int, ctypes.c_int]
         L.dpdf_resample.argtypes = [ctypes.c_int, vp, ctypes.c_int, ctypes.c_long, ctypes.c_int, ctypes.c_int, vp, ctypes.c_int]
-        for op in (L.dpdf_gated_delta, L.dpdf_gated_delta_step, L.dpdf_w4_quantize, L.dpdf_w4_matvec):
+        L.dpdf_gated_delta_workspace.restype = ctypes.c_size_t
+        L.dpdf_gated_delta_workspace.argtypes = [ctypes.c_int, vp]
+        L.dpdf_gated_delta.argtypes = [ctypes.c_int, vp, vp, ctypes.c_size_t, vp]
+        for op in (L.dpdf_gated_delta_step, L.dpdf_w4_quantize, L.dpdf_w4_matvec):
             op.argtypes = [ctypes.c_int, vp, vp]
         _lib = L
         return L

@@ -20,6 +20,9 @@ struct GatedDeltaArgs {
     int strips;                       // workgroups (clip) or waves (step) per head
     int gate;                         // type of g and beta: 0 fp32, 1 fp16, 2 bf16
     int whole;                        // clips: k and q can be read in pieces of eight values
+    int segments, seg;                // clips: how many pieces a clip is cut into, and their frames
+    float* starts;                    // [segments][B Hv][Dk][Dv]: the states that segments 1 .. start with; before they are joined, what each adds
+    float* moves;                     // [segments][B Hv][Dk][Dk]: segment i's effect on the state before it, i = 1 .. segments - 2
     float scale;
 };
 
@@ -139,6 +142,11 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
 // term) left out; bf16 values of k and q are one limb, fp16 two, fp32 three.  What only reaches the outputs of a 16-bit type (Q S, P u) takes two
 // limbs of either side, 2^-16 of a term against the 2^-8 and 2^-11 of the result's rounding; the state's path takes all.
 //
+// Where there are fewer heads than the chip holds workgroups, the frames are cut into segments.  A segment's effect on the state before it is
+// linear, S -> M S + N: MOVE runs a segment from S = 0 with its v (N) and from the unit matrix without (M, Dk columns more), no outputs;
+// gated_delta_join_kernel then walks the segments (N becomes the state that the next one starts with), and the segments run as
+// clips of their own.  About two and a half times the work, over `segments` times the workgroups.
+//
 // gamma and its differences are 64-bit: they are small differences of long sums.  A non-finite k, g or beta makes its head's outputs from its
 // frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all
 // frames of the chunk, so that such values are taken out of the operands first).
@@ -247,7 +255,7 @@ template <int N> __device__ __forceinline__ f32x4 gd_mul16(const uint2 (&a)[N], 
     return mfma_bf16(a01, gd_two(b[0], b[0]), acc);
 }
 
-template <typename T, int DKP, int NW, int C>
+template <typename T, int DKP, int NW, int C, bool MOVE>
 __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDeltaArgs a) {
     constexpr int L = GdIn<T>::L, NB = DKP / 16, NC = DKP / 32, CB = C / 16, CC = C / 32, LDK = DKP + 8, LDT = C + 8, E = sizeof(T);
     constexpr int BLOCKS = CB * (CB + 1) / 2;
@@ -255,32 +263,41 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
     constexpr int PL = WIDE ? 3 : 2, ITEMS = (C / 2 * (DKP / 8) + 64 * NW - 1) / (64 * NW);
     // blocks of A below the diagonal and of P on and below it, two neighbours of a row to a fragment: row bi of A starts at bi^2 / 4, of P at (bi + 1)^2 / 4
     constexpr int ASLOTS = CB * CB / 4, PSLOTS = (CB + 1) * (CB + 1) / 4;
-    __shared__ __attribute__((aligned(16))) unsigned short Kr[L][C][LDK], Qr[L][C][LDK], Kt[L][DKP][LDT];
-    __shared__ __attribute__((aligned(16))) uint2 Af[ASLOTS][3][64][2], Pf[PSLOTS][PL][64][2];
+    __shared__ __attribute__((aligned(16))) unsigned short Kr[L][C][LDK], Qr[MOVE ? 1 : L][MOVE ? 1 : C][LDK], Kt[L][DKP][LDT];
+    __shared__ __attribute__((aligned(16))) uint2 Af[ASLOTS][3][64][2], Pf[MOVE ? 1 : PSLOTS][PL][64][2];
     __shared__ __attribute__((aligned(16))) float Ad[CB][16][20];
     __shared__ __attribute__((aligned(16))) float2 gam[C];
     __shared__ __attribute__((aligned(16))) float eg[C], ee[C], bt[C];
     __shared__ int kbad[2];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
-    const long head = blockIdx.x / a.strips;
+    const long unit = blockIdx.x / a.strips;               // (head, segment)
+    const int sg = (int)(unit % a.segments);
+    const long head = unit / a.segments, heads = (long)(gridDim.x / a.strips) / a.segments;
     const int b = (int)(head / a.Hv), h = (int)(head - (long)b * a.Hv), hk = h / (a.Hv / a.Hk);
-    const int c0w = 16 * NW * (int)(blockIdx.x - head * a.strips) + 16 * w, col = c0w + n;
-    const bool cin = col < a.Dv;
+    int col = 16 * NW * (int)(blockIdx.x - unit * a.strips) + 16 * w + n;
+    const int vcols = (a.Dv + 15) & ~15;
+    const bool eye = MOVE && col >= vcols;                 // a column of the unit matrix: the same for a wave
+    if (MOVE && (sg == a.segments - 1 || (sg == 0 && 16 * NW * (int)(blockIdx.x - unit * a.strips) >= vcols))) return;
+    if (eye) col -= vcols;
+    const bool cin = col < (eye ? a.Dk : a.Dv);
     int len = a.lengths ? a.lengths[b] : a.T;
     len = len < 0 ? 0 : len > a.T ? a.T : len;
+    const int first = sg * a.seg;
+    if (len - first > a.seg) len = first + a.seg;          // the segment's end
     const long qb = (long)b * a.qs[0] + (long)hk * a.qs[2], kb = (long)b * a.ks[0] + (long)hk * a.ks[2];
     const long vb = (long)b * a.vs[0] + (long)h * a.vs[2], ob = (long)b * a.os[0] + (long)h * a.os[2];
     const long gb = (long)b * a.gs[0] + (long)h * a.gs[2], bb = (long)b * a.bs[0] + (long)h * a.bs[2];
     const long sb = head * a.Dk * a.Dv + col;
+    const float* from = sg == 0 ? a.state_in : MOVE ? nullptr : a.starts + (long)sg * heads * a.Dk * a.Dv;
     const unsigned vstep = (unsigned)a.vs[1] * E, ostep = (unsigned)a.os[1] * E;
-    const unsigned voff = cin ? 4 * q * vstep + col * E : GD_OUT, ooff = cin ? 4 * q * ostep + col * E : GD_OUT;
+    const unsigned voff = cin && !eye ? 4 * q * vstep + col * E : GD_OUT, ooff = cin ? 4 * q * ostep + col * E : GD_OUT;
     f32x4 S[NB];
 #pragma unroll
     for (int c = 0; c < NB; ++c)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = 16 * c + 4 * q + i;
-            S[c][i] = a.state_in && cin && r < a.Dk ? a.state_in[sb + (long)r * a.Dv] : 0.f;
+            S[c][i] = eye ? (r == col ? 1.f : 0.f) : from && cin && r < a.Dk ? from[sb + (long)r * a.Dv] : 0.f;
         }
 
     // a chunk on its way: two rows of eight k and q per item, this lane's v, the gates of frame `lane`
@@ -298,7 +315,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 nk[it][x] = gd_row<T>(rk, (2 * p + x) * (unsigned)a.ks[1] * E + 8 * j * E, a.Dk - 8 * j, whole);
-                nq[it][x] = gd_row<T>(rq, (2 * p + x) * (unsigned)a.qs[1] * E + 8 * j * E, a.Dk - 8 * j, whole);
+                if constexpr (!MOVE) nq[it][x] = gd_row<T>(rq, (2 * p + x) * (unsigned)a.qs[1] * E + 8 * j * E, a.Dk - 8 * j, whole);
             }
         }
 #pragma unroll
@@ -312,8 +329,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
         }
     };
     if (tid < 2) kbad[tid] = C;
-    if (len > 0) fetch(0);
-    for (int t0 = 0, par = 0; t0 < len; t0 += C, par ^= 1) {
+    if (len > first) fetch(first);
+    for (int t0 = first, par = 0; t0 < len; t0 += C, par ^= 1) {
         const int m = len - t0 < C ? len - t0 : C;
         __syncthreads();
 #pragma unroll
@@ -328,7 +345,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
                     for (int l = 0; l < L; ++l) kl[x][l] = make_uint4(0, 0, 0, 0);
                 }
-                gd_limbs<T>(nq[it][x], ql[x]);
+                if constexpr (!MOVE) gd_limbs<T>(nq[it][x], ql[x]);
             }
             const int c0 = 32 * (j >> 2) + 8 * (2 * j & 3) + 4 * (j >> 1 & 1);                    // slots of k 8 j .. 8 j + 3; the next four are 8 on
             const int r0 = 2 * p, tc = 32 * (r0 >> 5) + 8 * (r0 >> 2 & 3) + 4 * (r0 >> 4 & 1) + (r0 & 3);
@@ -337,6 +354,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     *(uint2*)&Kr[l][r0 + x][c0] = make_uint2(kl[x][l].x, kl[x][l].y); *(uint2*)&Kr[l][r0 + x][c0 + 8] = make_uint2(kl[x][l].z, kl[x][l].w);
+                    if constexpr (MOVE) continue;
                     *(uint2*)&Qr[l][r0 + x][c0] = make_uint2(ql[x][l].x, ql[x][l].y); *(uint2*)&Qr[l][r0 + x][c0 + 8] = make_uint2(ql[x][l].z, ql[x][l].w);
                 }
                 const unsigned u0[4] = {kl[0][l].x, kl[0][l].y, kl[0][l].z, kl[0][l].w}, u1[4] = {kl[1][l].x, kl[1][l].y, kl[1][l].z, kl[1][l].w};
@@ -380,10 +398,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 for (int l = 0; l < L; ++l) {
                     kj[l] = *(const uint4*)&Kr[l][16 * bj + n][32 * c + 8 * q];
                     ki[l] = *(const uint4*)&Kr[l][16 * bi + n][32 * c + 8 * q];
-                    qi[l] = *(const uint4*)&Qr[l][16 * bi + n][32 * c + 8 * q];
+                    if constexpr (!MOVE) qi[l] = *(const uint4*)&Qr[l][16 * bi + n][32 * c + 8 * q];
                 }
                 xa = gd_mul<2>(kj, ki, xa);
-                xp = gd_mul<2>(kj, qi, xp);
+                if constexpr (!MOVE) xp = gd_mul<2>(kj, qi, xp);
             }
             const float2 gr = gam[16 * bi + n];
             const float br = -bt[16 * bi + n];
@@ -408,6 +426,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
                 for (int l = 0; l < 3; ++l) Af[bi * bi / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
             }
+            if constexpr (MOVE) continue;
             uint4 f[PL];
             gd_split(xp, f, 0);
 #pragma unroll
@@ -441,9 +460,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 for (int c = 0; c < NC; ++c) {
                     uint4 kf[L], qf[L];
 #pragma unroll
-                    for (int l = 0; l < L; ++l) { kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q]; qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q]; }
+                    for (int l = 0; l < L; ++l) { kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q]; if constexpr (!MOVE) qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q]; }
                     x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
-                    y[bl] = gd_mul<WIDE ? 2 : 1>(qf, sl[c], y[bl]);
+                    if constexpr (!MOVE) y[bl] = gd_mul<WIDE ? 2 : 1>(qf, sl[c], y[bl]);
                 }
             }
         }
@@ -458,7 +477,6 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             { const int z = __shfl_xor(bad, 16); bad = z < bad ? z : bad; }
             { const int z = __shfl_xor(bad, 32); bad = z < bad ? z : bad; }
         }
-        const auto ro = gd_buffer(a.out, ob + (long)t0 * a.os[1], (m - 1) * a.os[1] + a.Dv, E);
         uint4 ul[CC][3], wl[CC][3];
         f32x4 o[CB];
 #pragma unroll
@@ -484,19 +502,21 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             f32x4 u = {0.f, 0.f, 0.f, 0.f};
             u = mfma16(t.x, z[0], u); u = mfma16(t.y, z[1], u); u = mfma16(t.z, z[2], u); u = mfma16(t.w, z[3], u);
             gd_split(u, ul[bl / 2], bl & 1);
-            o[bl][0] = a.scale * e4.x * y[bl][0]; o[bl][1] = a.scale * e4.y * y[bl][1]; o[bl][2] = a.scale * e4.z * y[bl][2]; o[bl][3] = a.scale * e4.w * y[bl][3];
+            if constexpr (!MOVE) {
+                o[bl][0] = a.scale * e4.x * y[bl][0]; o[bl][1] = a.scale * e4.y * y[bl][1]; o[bl][2] = a.scale * e4.z * y[bl][2]; o[bl][3] = a.scale * e4.w * y[bl][3];
 #pragma unroll
-            for (int c = 0; c < (bl + 1) / 2; ++c) {
-                uint4 f[PL];
+                for (int c = 0; c < (bl + 1) / 2; ++c) {
+                    uint4 f[PL];
 #pragma unroll
-                for (int l = 0; l < PL; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
-                o[bl] = gd_mul<PL - 1>(f, ul[c], o[bl]);
-            }
-            if (!(bl & 1)) {
-                uint2 f[PL];
+                    for (int l = 0; l < PL; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
+                    o[bl] = gd_mul<PL - 1>(f, ul[c], o[bl]);
+                }
+                if (!(bl & 1)) {
+                    uint2 f[PL];
 #pragma unroll
-                for (int l = 0; l < PL; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
-                o[bl] = gd_mul16(f, ul[bl / 2], o[bl]);
+                    for (int l = 0; l < PL; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
+                    o[bl] = gd_mul16(f, ul[bl / 2], o[bl]);
+                }
             }
             u[0] *= f4.x; u[1] *= f4.y; u[2] *= f4.z; u[3] *= f4.w;
             gd_split(u, wl[bl / 2], bl & 1);
@@ -524,17 +544,72 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 for (int i = 0; i < 4; ++i)
                     if (16 * bl + 4 * q + i >= bad) o[bl][i] = z;
         }
+        if constexpr (!MOVE) {
+            const auto ro = gd_buffer(a.out, ob + (long)t0 * a.os[1], (m - 1) * a.os[1] + a.Dv, E);
 #pragma unroll
-        for (int bl = 0; bl < CB; ++bl)
+            for (int bl = 0; bl < CB; ++bl)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) gd_put<T>(ro, ooff + (16 * bl + i) * ostep, o[bl][i]);
+                for (int i = 0; i < 4; ++i) gd_put<T>(ro, ooff + (16 * bl + i) * ostep, o[bl][i]);
+        }
     }
-    if (a.state_out && cin)
+    float* to = MOVE ? (eye ? a.moves + ((long)sg * heads + head) * a.Dk * a.Dk + col : a.starts + (long)(sg + 1) * heads * a.Dk * a.Dv + sb)
+                     : sg == a.segments - 1 && a.state_out ? a.state_out + sb : nullptr;
+    if (to && cin)
 #pragma unroll
         for (int c = 0; c < NB; ++c)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int r = 16 * c + 4 * q + i;
-                if (r < a.Dk) a.state_out[sb + (long)r * a.Dv] = S[c][i];
+                if (r < a.Dk) to[(long)r * (eye ? a.Dk : a.Dv)] = S[c][i];
             }
+}
+
+// The segments' states one after the other, S <- M S + N on the fp32 matrix instruction: a workgroup is 16 columns of a head, wave c its rows
+// 16 c .. 16 c + 15; the state goes round through LDS.
+template <int DKP>
+__global__ __launch_bounds__(4 * DKP) void gated_delta_join_kernel(GatedDeltaArgs a, long heads) {
+    constexpr int NB = DKP / 16;
+    __shared__ __attribute__((aligned(16))) float Sx[2][16][DKP + 4];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+    const long head = blockIdx.x / a.strips;
+    const int col = 16 * (int)(blockIdx.x - head * a.strips) + n, row = 16 * w + 4 * q;
+    const bool cin = col < a.Dv;
+    const long step = heads * a.Dk * a.Dv, sb = head * a.Dk * a.Dv + col;
+    const int mrow = 16 * w + n < a.Dk ? 16 * w + n : a.Dk - 1;          // what lies behind Dk is 0 on the other side, and not written
+    const float* mv = a.moves + (head * a.Dk + mrow) * a.Dk;
+    const long mstep = heads * a.Dk * a.Dk;
+    auto piece = [&](int s, float (&x)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = cin && row + i < a.Dk ? a.starts[(long)s * step + sb + (long)(row + i) * a.Dv] : 0.f;
+    };
+    auto matrix = [&](int s, float (&x)[NB][4]) {
+#pragma unroll
+        for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[c][i] = 16 * c + 4 * q + i < a.Dk ? mv[(long)s * mstep + 16 * c + 4 * q + i] : 0.f;
+    };
+    float x[4], nx[4], m[NB][4];
+    piece(1, x);
+    if (a.segments > 2) { matrix(1, m); piece(2, nx); }
+    for (int s = 1; s + 1 < a.segments; ++s) {
+        *(float4*)&Sx[s & 1][n][row] = make_float4(x[0], x[1], x[2], x[3]);
+        __syncthreads();
+        f32x4 y = {nx[0], nx[1], nx[2], nx[3]};
+        float cm[NB][4];
+#pragma unroll
+        for (int c = 0; c < NB; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cm[c][i] = m[c][i];
+        if (s + 2 < a.segments) { matrix(s + 1, m); piece(s + 2, nx); }
+#pragma unroll
+        for (int c = 0; c < NB; ++c) {
+            const float4 v = *(const float4*)&Sx[s & 1][n][16 * c + 4 * q];
+            y = mfma16(cm[c][0], v.x, y); y = mfma16(cm[c][1], v.y, y); y = mfma16(cm[c][2], v.z, y); y = mfma16(cm[c][3], v.w, y);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] = row + i < a.Dk ? y[i] : 0.f;
+            if (cin && row + i < a.Dk) a.starts[(long)(s + 1) * step + sb + (long)(row + i) * a.Dv] = y[i];
+        }
+    }
 }

@@ -1,9 +1,6 @@
 // host_operators.h -- C entry points of the stand-alone operators (gated_delta.h, w4_matvec.h): device pointers, the caller's stream, nothing
 // allocated, nothing waited for, so that every call can be captured into a graph.  Arguments are checked before anything is launched.
 
-#ifndef GD_CHUNK
-#define GD_CHUNK 64
-#endif
 namespace {
 struct OpDevice {                                 // the call's device for as long as it runs, the caller's afterwards
     int before = -1; hipError_t err;
@@ -45,6 +42,7 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
     const int e = op_bytes(x.dtype), ge = op_bytes(x.gate_dtype);
     if (!e || !ge || (x.gate_dtype != DPDF_F32 && x.gate_dtype != x.dtype)) return set_err(DPDF_E_INVALID, "gated delta rule: unsupported dtypes %d / %d", x.dtype, x.gate_dtype);
     if (x.batch < 0 || x.frames < 0) return set_err(DPDF_E_INVALID, "gated delta rule: negative size batch=%d frames=%d", x.batch, x.frames);
+    if (x.frames > 1 << 30) return set_err(DPDF_E_INVALID, "gated delta rule: %d frames are too large a number for one call", x.frames);
     if (x.k_heads < 1 || x.v_heads < 1 || x.v_heads % x.k_heads) return set_err(DPDF_E_INVALID, "gated delta rule: %d value heads are no multiple of %d key heads", x.v_heads, x.k_heads);
     if (x.k_dim < 1 || x.k_dim > 128 || x.v_dim < 1) return set_err(DPDF_E_INVALID, "gated delta rule: head sizes %d (1 .. 128) and %d (from 1)", x.k_dim, x.v_dim);
     if (!(x.scale - x.scale == 0.f)) return set_err(DPDF_E_INVALID, "gated delta rule: scale is not finite");
@@ -79,6 +77,7 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
         a.gs[i] = x.g_stride[i]; a.bs[i] = x.beta_stride[i]; a.os[i] = x.out_stride[i];
     }
     a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale; a.gate = x.gate_dtype;
+    a.segments = 1; a.seg = 0; a.starts = a.moves = nullptr; a.whole = 0; a.strips = 0;
     return DPDF_OK;
 }
 
@@ -88,14 +87,40 @@ void gd_launch_step(const GatedDeltaArgs& a, unsigned grid, bool even, hipStream
     if (a.Dk <= 16) GD_STEP(16); else if (a.Dk <= 32) GD_STEP(32); else if (a.Dk <= 64) GD_STEP(64); else GD_STEP(128);
 #undef GD_STEP
 }
-template <typename T, int NW>
+// The frames of a chunk, the columns of a workgroup and the workgroups that a CU holds at once (registers and LDS)
+int gd_chunk(int dtype) { return dtype == DPDF_F32 ? 32 : 64; }
+int gd_columns(const GatedDeltaArgs& a) { return a.Dv <= 64 ? 64 : 128; }
+int gd_resident(const GatedDeltaArgs& a) { return a.Dv <= 64 && a.Dk <= 64 ? 2 : 1; }
+// Segments for `heads` heads: as many as fill the chip once, with four chunks at least each (their start state costs about one and a half times
+// their frames), and only where the chip would hold three times the workgroups there are.
+int gd_segments(const GatedDeltaArgs& a, long heads, int chunk, int cus) {
+    const long strips = (a.Dv + gd_columns(a) - 1) / gd_columns(a), groups = heads * strips, room = (long)cus * gd_resident(a);
+    const long chunks = ((long)a.T + chunk - 1) / chunk;
+    long n = room / groups;
+    if (n > chunks / 4) n = chunks / 4;
+    return n < 3 ? 1 : (int)n;
+}
+size_t gd_workspace(const GatedDeltaArgs& a, long heads, int segments) {
+    return segments < 2 ? 0 : (size_t)segments * heads * a.Dk * (a.Dk + a.Dv) * sizeof(float);
+}
+template <typename T, int DKP, int NW>
 void gd_launch_clip(GatedDeltaArgs& a, long heads, hipStream_t s) {
+    constexpr int C = sizeof(T) == 4 ? 32 : 64;
+    const long units = heads * a.segments, vcols = (a.Dv + 15) & ~15, kcols = (a.Dk + 15) & ~15;
+    if (a.segments > 1) {
+        a.strips = (int)((vcols + kcols + 16 * NW - 1) / (16 * NW));
+        gated_delta_clip_kernel<T, DKP, NW, C, true><<<(unsigned)(units * a.strips), 64 * NW, 0, s>>>(a);
+        a.strips = (int)(vcols / 16);
+        gated_delta_join_kernel<DKP><<<(unsigned)(heads * a.strips), 4 * DKP, 0, s>>>(a, heads);
+    }
     a.strips = (a.Dv + 16 * NW - 1) / (16 * NW);
-    const unsigned grid = (unsigned)(heads * a.strips);
-    constexpr int C = sizeof(T) == 4 ? 32 : GD_CHUNK;
-    if (a.Dk <= 32) gated_delta_clip_kernel<T, 32, NW, C><<<grid, 64 * NW, 0, s>>>(a);
-    else if (a.Dk <= 64) gated_delta_clip_kernel<T, 64, NW, C><<<grid, 64 * NW, 0, s>>>(a);
-    else gated_delta_clip_kernel<T, 128, NW, C><<<grid, 64 * NW, 0, s>>>(a);
+    gated_delta_clip_kernel<T, DKP, NW, C, false><<<(unsigned)(units * a.strips), 64 * NW, 0, s>>>(a);
+}
+template <typename T>
+void gd_launch_clips(GatedDeltaArgs& a, long heads, hipStream_t s) {
+#define GD_CLIP(D) (gd_columns(a) == 64 ? gd_launch_clip<T, D, 4>(a, heads, s) : gd_launch_clip<T, D, 8>(a, heads, s))
+    if (a.Dk <= 32) GD_CLIP(32); else if (a.Dk <= 64) GD_CLIP(64); else GD_CLIP(128);
+#undef GD_CLIP
 }
 template <typename F> void gd_type(int dtype, F f) {
     if (dtype == DPDF_F32) f(float()); else if (dtype == DPDF_F16) f(__half()); else f(__hip_bfloat16());
@@ -126,23 +151,47 @@ int w4_check(int dtype, long K, long N, int group, const char* what) {
 }
 }  // namespace
 
-extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* stream) {
+extern "C" size_t dpdf_gated_delta_workspace(int device, const dpdf_gated_delta_args* args) {
+    GatedDeltaArgs a;
+    int cus = 0;
+    if (gd_check(args, false, a) || !args->batch || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) return 0;
+    const long heads = (long)args->batch * a.Hv;
+    return gd_workspace(a, heads, gd_segments(a, heads, gd_chunk(args->dtype), cus));
+}
+
+extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* workspace, size_t workspace_bytes, void* stream) {
     GatedDeltaArgs a;
     if (int rc = gd_check(args, false, a)) return rc;
     if (!args->batch || (!args->frames && !args->state_out)) return DPDF_OK;
     // a chunk's rows are addressed with 32 bits
-    const long most = (1L << 31) - 1, rows = args->frames < 1 ? 1 : args->frames < GD_CHUNK ? args->frames : GD_CHUNK, e = op_bytes(args->dtype);
+    const long most = (1L << 31) - 1, rows = args->frames < 1 ? 1 : args->frames < 64 ? args->frames : 64, e = op_bytes(args->dtype);
     for (const long* s : {args->q_stride, args->k_stride, args->v_stride, args->out_stride})
         if (s[1] > (most - (long)(a.Dk > a.Dv ? a.Dk : a.Dv) * e) / (rows * e)) return set_err(DPDF_E_INVALID, "gated delta rule: a stride of %ld from frame to frame is too large", s[1]);
+    if (!op_aligned(workspace, 16)) return set_err(DPDF_E_INVALID, "gated delta rule: the workspace is not aligned to 16 bytes");
     a.whole = a.Dk % 8 == 0;
     for (const void* p : {a.q, a.k}) a.whole &= op_aligned(p, 4);
     for (const long* s : {a.qs, a.ks}) for (int i = 0; i < 3; ++i) a.whole &= s[i] * e % 4 == 0;
     OpDevice dev(device);
     HIP_TRY(dev.err);
-    gd_type(args->dtype, [&](auto t) {
-        if (a.Dv <= 64) gd_launch_clip<decltype(t), 4>(a, (long)args->batch * a.Hv, (hipStream_t)stream);
-        else gd_launch_clip<decltype(t), 8>(a, (long)args->batch * a.Hv, (hipStream_t)stream);
-    });
+    const long heads = (long)args->batch * a.Hv, chunk = gd_chunk(args->dtype);
+    a.segments = 1; a.seg = (int)((args->frames + chunk - 1) / chunk * chunk);
+    if (workspace) {
+        int cus = 0;
+        HIP_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
+        const int n = gd_segments(a, heads, (int)chunk, cus);
+        if (n > 1 && workspace_bytes >= gd_workspace(a, heads, n)) {
+            const long chunks = (args->frames + chunk - 1) / chunk, each = (chunks + n - 1) / n;
+            a.seg = (int)(each * chunk); a.segments = (int)((chunks + each - 1) / each);
+            const OpSpan ws = {(const char*)workspace, (const char*)workspace + gd_workspace(a, heads, a.segments)};
+            const long B = args->batch, T = args->frames, kd[3] = {B, T, a.Hk}, vd[3] = {B, T, a.Hv}, ge = op_bytes(args->gate_dtype), state = heads * a.Dk * a.Dv * 4;
+            const OpSpan other[8] = {op_span(a.q, a.qs, kd, 3, a.Dk, e), op_span(a.k, a.ks, kd, 3, a.Dk, e), op_span(a.v, a.vs, vd, 3, a.Dv, e), op_span(a.out, a.os, vd, 3, a.Dv, e),
+                                     op_span(a.g, a.gs, vd, 3, 1, ge), op_span(a.beta, a.bs, vd, 3, 1, ge),
+                                     {(const char*)a.state_in, (const char*)a.state_in + (a.state_in ? state : 0)}, {(const char*)a.state_out, (const char*)a.state_out + (a.state_out ? state : 0)}};
+            for (const OpSpan& o : other) if (op_meet(ws, o)) return set_err(DPDF_E_INVALID, "gated delta rule: the workspace overlaps a tensor");
+            a.starts = (float*)workspace; a.moves = a.starts + (size_t)a.segments * heads * a.Dk * a.Dv;
+        }
+    }
+    gd_type(args->dtype, [&](auto t) { gd_launch_clips<decltype(t)>(a, heads, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());
     return DPDF_OK;
 }

@@ -3,7 +3,7 @@ hop, and dense layers with 4-bit weights for a few rows -- the parts of a recurr
 `dpdf_gated_delta_step`, `dpdf_w4_matvec`, `dpdf_w4_quantize` of include/dpdfnet_hip.h).
 
 Tensors are torch tensors on one HIP device, float32, float16 or bfloat16; calls are queued on torch's current stream of that device,
-allocate nothing beside their results and wait for nothing, so they can be captured into a graph.  Sums, states and accumulators are fp32
+allocate nothing beside their results (and, for a few long clips, a workspace) through torch and wait for nothing, so they can be captured into a graph.  Sums, states and accumulators are fp32
 whatever the tensors' type.  There is no backward pass: tensors that require a gradient are refused while gradients are recorded.  Wrong
 types, shapes and overlaps raise ValueError, failures of the device RuntimeError."""
 from __future__ import annotations
@@ -79,9 +79,9 @@ def _checked(device, shape, dtype, name: str, t):
     return t
 
 
-def _call(fn, device, args) -> None:
+def _call(fn, device, args, *workspace) -> None:
     stream = _torch().cuda.current_stream(device).cuda_stream
-    _backend._check(getattr(_backend.load_library(), fn)(device.index, ctypes.addressof(args), stream))
+    _backend._check(getattr(_backend.load_library(), fn)(device.index, ctypes.addressof(args), *workspace, stream))
 
 
 def _gated(fn, q, k, v, g, beta, state_in, state_out, lengths, active, scale, out):
@@ -120,7 +120,12 @@ def _gated(fn, q, k, v, g, beta, state_in, state_out, lengths, active, scale, ou
                         q.stride()[:3], k.stride()[:3], v.stride()[:3], g.stride(), beta.stride(), out.stride()[:3],
                         state_in.data_ptr() if state_in is not None else None, state_out.data_ptr() if state_out is not None else None,
                         lengths.data_ptr() if lengths is not None else None, active.data_ptr() if active is not None else None)
-    _call(fn, dev, a)
+    if fn == "dpdf_gated_delta_step":
+        _call(fn, dev, a)
+    else:
+        need = _backend.load_library().dpdf_gated_delta_workspace(dev.index, ctypes.addressof(a))
+        room = torch.empty(need, device=dev, dtype=torch.uint8) if need else None        # given back to torch when the call is queued: this stream's next users follow it
+        _call(fn, dev, a, room.data_ptr() if need else None, need)
     return out
 
 

@@ -103,7 +103,7 @@ def test_operators_are_reachable_under_both_names():
     assert set(operators.__all__) == {"gated_delta", "gated_delta_step", "w4_matvec", "w4_quantize"}
 
 
-def _c_gated(step=False, **change):
+def _c_gated(step=False, workspace=None, **change):
     """A call of the C entry on made-up addresses with one thing changed: refused before any of them is looked at."""
     B, T, Hk, Hv, Dk, Dv = 2, 3, 2, 4, 16, 8
     v = dict(dtype=2, gate_dtype=0, batch=B, frames=T, k_heads=Hk, v_heads=Hv, k_dim=Dk, v_dim=Dv, scale=1.0,
@@ -114,7 +114,7 @@ def _c_gated(step=False, **change):
     v.update(change)
     a = operators._GatedDeltaArgs(*[v[f[0]] for f in operators._GatedDeltaArgs._fields_])
     L = backend.load_library()
-    rc = (L.dpdf_gated_delta_step if step else L.dpdf_gated_delta)(0, ctypes.addressof(a), None)
+    rc = L.dpdf_gated_delta_step(0, ctypes.addressof(a), None) if step else L.dpdf_gated_delta(0, ctypes.addressof(a), workspace, 1 << 20, None)
     return rc, L.dpdf_last_error().decode()
 
 
@@ -126,7 +126,8 @@ def _c_gated(step=False, **change):
     (dict(q_stride=(-1, 1, 1)), "negative stride"), (dict(out_stride=(0, 32, 8)), "share"), (dict(out_stride=(96, 32, 7)), "share"), (dict(out_stride=(96, 24, 8)), "share"),
     (dict(out=0x3000000), "overlaps an input"), (dict(out=0x1000000 - 2), "overlaps an input"), (dict(out=0x7000000), "out overlaps"),
     (dict(state_out=0x7000004), "in part"), (dict(state_out=0x2000000), "overlaps an input"), (dict(active=0x9000000), "mask"),
-    (dict(batch=1 << 30), "too large"), (dict(k=1 << 45, k_stride=(1 << 38, 1 << 30, 16)), "frame to frame"), (dict(out=1 << 45, out_stride=(1 << 40, 1 << 31, 8)), "frame to frame"),
+    (dict(batch=1 << 30), "too large"), (dict(frames=(1 << 30) + 1), "too large"), (dict(workspace=0x9000008), "aligned"),
+ (dict(k=1 << 45, k_stride=(1 << 38, 1 << 30, 16)), "frame to frame"), (dict(out=1 << 45, out_stride=(1 << 40, 1 << 31, 8)), "frame to frame"),
 ])
 def test_gated_delta_refusals(change, word):
     rc, msg = _c_gated(**change)
@@ -137,7 +138,7 @@ def test_gated_delta_step_refusals_and_empty_calls():
     assert _c_gated(step=True, lengths=0x8000000)[0] == -1
     assert _c_gated(step=True, state_in=None)[0] == -1 and _c_gated(step=True, state_out=None)[0] == -1
     L = backend.load_library()
-    assert L.dpdf_gated_delta(0, None, None) == -1 and L.dpdf_gated_delta_step(0, None, None) == -1
+    assert L.dpdf_gated_delta(0, None, None, 0, None) == -1 and L.dpdf_gated_delta_workspace(0, None) == 0 and L.dpdf_gated_delta_step(0, None, None) == -1
     assert L.dpdf_w4_matvec(0, None, None) == -1 and L.dpdf_w4_quantize(0, None, None) == -1
     # nothing to do: no device is touched
     assert _c_gated(batch=0)[0] == 0 and _c_gated(step=True, batch=0)[0] == 0 and _c_gated(step=True, frames=0)[0] == 0
@@ -432,6 +433,55 @@ def test_large_and_small_values_keep_their_precision(dtype):
     for c in range(64):
         near(out[..., c], ref[..., c], tol(100, 64), HALF_STEP[dtype], TINY[dtype])
         near(end[..., c], rend[..., c], tol(100, 64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T, lens, Hk, Hv, Dk, Dv", [(1200, None, 1, 2, 64, 64), (2000, (2000, 777), 1, 1, 16, 40), (1500, (0, 1500), 2, 2, 128, 128), (900, (64, 899), 1, 2, 48, 20),
+                                                     (1030, None, 1, 1, 100, 100)])
+def test_few_long_clips_are_cut_into_segments(T, lens, Hk, Hv, Dk, Dv, dtype):
+    """Against the definition, and against the same call without a workspace (one piece)."""
+    B = 2
+    x = inputs(B, T, Hk, Hv, Dk, Dv, dtype, seed=T, g_std=3.0)        # heads that remember a few frames beside heads that remember all
+    x[3][0, T // 2] = -math.inf
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    state = 0.5 * torch.randn(B, Hv, Dk, Dv, generator=torch.Generator().manual_seed(1)).cuda()
+    ref, rend = delta_rule(*x, state=state, lengths=lengths)
+    out, end = operators.gated_delta(*x, state=state, lengths=lengths)
+    near(out, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
+    near(end, rend, tol(T, Dk))
+    q, k, v, g, beta = x
+    L = backend.load_library()
+    out1, end1 = torch.zeros_like(out), torch.empty_like(end)
+    a = operators._GatedDeltaArgs({F32: 0, F16: 1, BF16: 2}[dtype], 0, B, T, Hk, Hv, Dk, Dv, 1 / math.sqrt(Dk), *[t.data_ptr() for t in x], out1.data_ptr(),
+                                  q.stride()[:3], k.stride()[:3], v.stride()[:3], g.stride(), beta.stride(), out1.stride()[:3],
+                                  state.data_ptr(), end1.data_ptr(), None if lens is None else lengths.data_ptr(), None)
+    assert L.dpdf_gated_delta_workspace(0, ctypes.addressof(a)) > 0
+    assert L.dpdf_gated_delta(0, ctypes.addressof(a), None, 0, torch.cuda.current_stream().cuda_stream) == 0
+    near(out1, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
+    near(end1, rend, tol(T, Dk))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["k", "v", "beta"])
+@pytest.mark.parametrize("at", [0, 700, 1199])
+def test_a_non_finite_value_in_a_clip_of_segments(what, at):
+    x = inputs(1, 1200, 1, 2, 32, 32, BF16, seed=11)
+    clean, cend = operators.gated_delta(*x)
+    y = [t.clone() for t in x]
+    if what == "beta":
+        y[4][0, at, 0] = math.nan
+    else:
+        y["q k v".split().index(what)][0, at, 0, 5] = math.inf
+    out, end = operators.gated_delta(*y)
+    hit, shit = torch.zeros_like(out, dtype=torch.bool), torch.zeros_like(end, dtype=torch.bool)
+    if what == "v":
+        hit[0, at:, 0, 5] = shit[0, 0, :, 5] = True
+    else:
+        heads = slice(0, 2) if what == "k" else slice(0, 1)          # both value heads read the key head
+        hit[0, at:, heads] = shit[0, heads] = True
+    assert torch.equal(out[~hit], clean[~hit]) and not bool(torch.isfinite(out[hit]).any())
+    assert torch.equal(end[~shit], cend[~shit]) and not bool(torch.isfinite(end[shit]).any())
 
 
 @pytest.mark.gpu
