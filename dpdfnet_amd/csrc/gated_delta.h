@@ -19,7 +19,7 @@ struct GatedDeltaArgs {
     int T, Hk, Hv, Dk, Dv;
     int strips;                       // workgroups (clip) or waves (step) per head
     int gate;                         // type of g and beta: 0 fp32, 1 fp16, 2 bf16
-    int whole;                        // clips: k and q can be read in pieces of eight values
+    int whole, even;                  // clips: k and q can be read in pieces of eight values, out written in pieces of four
     int segments, seg;                // clips: how many pieces a clip is cut into, and their frames
     float* starts;                    // [segments][B Hv][Dk][Dv]: the states that segments 1 .. start with; before they are joined, what each adds
     float* moves;                     // [segments][B Hv][Dk][Dk]: segment i's effect on the state before it, i = 1 .. segments - 2
@@ -203,10 +203,29 @@ template <typename T> __device__ __forceinline__ float gd_value(unsigned raw) {
     else if constexpr (__is_same(T, __half)) return (float)__builtin_bit_cast(_Float16, (unsigned short)raw);
     else return __builtin_bit_cast(float, raw);
 }
-template <typename T> __device__ __forceinline__ void gd_put(__amdgpu_buffer_rsrc_t r, unsigned off, float v) {
-    if constexpr (__is_same(T, __hip_bfloat16)) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (__bf16)v), r, off, 0, 0);
-    else if constexpr (__is_same(T, __half)) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, (_Float16)v), r, off, 0, 0);
-    else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), r, off, 0, 0);
+// four columns of a row, `left` of them inside (even: in one piece)
+template <typename T> __device__ __forceinline__ void gd_put(__amdgpu_buffer_rsrc_t r, unsigned off, const f32x4& v, int left, bool even) {
+    if constexpr (sizeof(T) == 4) {
+        if (even) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(gd_u4, v), r, left > 0 ? off : GD_OUT, 0, 0);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = v[i];                      // a bit cast of v[i] itself takes element 0
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x), r, i < left ? off + 4 * i : GD_OUT, 0, 0);
+            }
+    } else {
+        typedef unsigned u2 __attribute__((ext_vector_type(2)));
+        u2 w;
+        if constexpr (__is_same(T, __hip_bfloat16)) w = (u2){pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+        else {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            w = (u2){__builtin_bit_cast(unsigned, (h2){(_Float16)v[0], (_Float16)v[1]}), __builtin_bit_cast(unsigned, (h2){(_Float16)v[2], (_Float16)v[3]})};
+        }
+        if (even) __builtin_amdgcn_raw_buffer_store_b64(w, r, left > 0 ? off : GD_OUT, 0, 0);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[i / 2] >> (16 * (i & 1))), r, i < left ? off + 2 * i : GD_OUT, 0, 0);
+    }
 }
 // the row's limbs, 8 x 16 bit each; true where a value is not finite
 template <typename T> __device__ __forceinline__ bool gd_limbs(const GdRow<T>& r, uint4 (&f)[GdIn<T>::L]) {
@@ -248,22 +267,42 @@ template <int TOP, int NA, int NB> __device__ __forceinline__ f32x4 gd_mul(const
 }
 // the same over 16 slots, those of the lower halves: two limbs of a side share a fragment
 __device__ __forceinline__ uint4 gd_two(const uint4& x, const uint4& y) { return make_uint4(x.x, x.y, y.x, y.y); }
-template <int N> __device__ __forceinline__ f32x4 gd_mul16(const uint2 (&a)[N], const uint4* b, f32x4 acc) {
+__device__ __forceinline__ f32x4 gd_mul16(const uint2 (&a)[3], const uint4* b, f32x4 acc) {
     const uint4 a01 = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
-    if constexpr (N == 3) acc = mfma_bf16(make_uint4(a[0].x, a[0].y, a[2].x, a[2].y), gd_two(b[2], b[0]), acc);
+    acc = mfma_bf16(make_uint4(a[0].x, a[0].y, a[2].x, a[2].y), gd_two(b[2], b[0]), acc);
     acc = mfma_bf16(a01, gd_two(b[1], b[1]), acc);
     return mfma_bf16(a01, gd_two(b[0], b[0]), acc);
+}
+// The transposes of such products: the two operands' layouts are the same, so the other order gives the transpose, a lane four columns of a row.
+template <int TOP, int NA, int NB> __device__ __forceinline__ f32x4 gd_mul_t(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 acc) {
+#pragma unroll
+    for (int o = TOP; o >= 0; --o)
+#pragma unroll
+        for (int l = 0; l < NA; ++l)
+            if (o - l >= 0 && o - l < NB) acc = mfma_bf16(b[o - l], a[l], acc);
+    return acc;
+}
+template <int N> __device__ __forceinline__ f32x4 gd_mul16_t(const uint2 (&a)[N], const uint4* b, f32x4 acc) {
+    const uint4 a01 = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
+    if constexpr (N == 3) acc = mfma_bf16(gd_two(b[2], b[0]), make_uint4(a[0].x, a[0].y, a[2].x, a[2].y), acc);
+    acc = mfma_bf16(gd_two(b[1], b[1]), a01, acc);
+    return mfma_bf16(gd_two(b[0], b[0]), a01, acc);
+}
+// four rows of a column out of rows in LDS: lane p of 16 gives the address of row p / 4, columns 4 (p % 4) .. + 3 and gets column p of all four
+typedef short gd_s4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 gd_column(const unsigned short* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) gd_s4*)p));
 }
 
 template <typename T, int DKP, int NW, int C, bool MOVE>
 __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDeltaArgs a) {
-    constexpr int L = GdIn<T>::L, NB = DKP / 16, NC = DKP / 32, CB = C / 16, CC = C / 32, LDK = DKP + 8, LDT = C + 8, E = sizeof(T);
+    constexpr int L = GdIn<T>::L, NB = DKP / 16, NC = DKP / 32, CB = C / 16, CC = C / 32, LDK = DKP + 8, E = sizeof(T);
     constexpr int BLOCKS = CB * (CB + 1) / 2;
     constexpr bool WIDE = E == 4;                          // outputs of 32 bits
     constexpr int PL = WIDE ? 3 : 2, ITEMS = (C / 2 * (DKP / 8) + 64 * NW - 1) / (64 * NW);
     // blocks of A below the diagonal and of P on and below it, two neighbours of a row to a fragment: row bi of A starts at bi^2 / 4, of P at (bi + 1)^2 / 4
     constexpr int ASLOTS = CB * CB / 4, PSLOTS = (CB + 1) * (CB + 1) / 4;
-    __shared__ __attribute__((aligned(16))) unsigned short Kr[L][C][LDK], Qr[MOVE ? 1 : L][MOVE ? 1 : C][LDK], Kt[L][DKP][LDT];
+    __shared__ __attribute__((aligned(16))) unsigned short Kr[L][C][LDK], Qr[MOVE ? 1 : L][MOVE ? 1 : C][LDK];
     __shared__ __attribute__((aligned(16))) uint2 Af[ASLOTS][3][64][2], Pf[MOVE ? 1 : PSLOTS][PL][64][2];
     __shared__ __attribute__((aligned(16))) float Ad[CB][16][20];
     __shared__ __attribute__((aligned(16))) float2 gam[C];
@@ -290,7 +329,9 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
     const long sb = head * a.Dk * a.Dv + col;
     const float* from = sg == 0 ? a.state_in : MOVE ? nullptr : a.starts + (long)sg * heads * a.Dk * a.Dv;
     const unsigned vstep = (unsigned)a.vs[1] * E, ostep = (unsigned)a.os[1] * E;
-    const unsigned voff = cin && !eye ? 4 * q * vstep + col * E : GD_OUT, ooff = cin ? 4 * q * ostep + col * E : GD_OUT;
+    const unsigned voff = cin && !eye ? 4 * q * vstep + col * E : GD_OUT;
+    const int ocol = col - n + 4 * q;                      // out: row n of a block, four columns
+    const unsigned ooff = n * ostep + ocol * E;
     f32x4 S[NB];
 #pragma unroll
     for (int c = 0; c < NB; ++c)
@@ -348,22 +389,15 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 if constexpr (!MOVE) gd_limbs<T>(nq[it][x], ql[x]);
             }
             const int c0 = 32 * (j >> 2) + 8 * (2 * j & 3) + 4 * (j >> 1 & 1);                    // slots of k 8 j .. 8 j + 3; the next four are 8 on
-            const int r0 = 2 * p, tc = 32 * (r0 >> 5) + 8 * (r0 >> 2 & 3) + 4 * (r0 >> 4 & 1) + (r0 & 3);
+            const int r0 = 2 * p;
 #pragma unroll
-            for (int l = 0; l < L; ++l) {
+            for (int l = 0; l < L; ++l)
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     *(uint2*)&Kr[l][r0 + x][c0] = make_uint2(kl[x][l].x, kl[x][l].y); *(uint2*)&Kr[l][r0 + x][c0 + 8] = make_uint2(kl[x][l].z, kl[x][l].w);
                     if constexpr (MOVE) continue;
                     *(uint2*)&Qr[l][r0 + x][c0] = make_uint2(ql[x][l].x, ql[x][l].y); *(uint2*)&Qr[l][r0 + x][c0 + 8] = make_uint2(ql[x][l].z, ql[x][l].w);
                 }
-                const unsigned u0[4] = {kl[0][l].x, kl[0][l].y, kl[0][l].z, kl[0][l].w}, u1[4] = {kl[1][l].x, kl[1][l].y, kl[1][l].z, kl[1][l].w};
-#pragma unroll
-                for (int d = 0; d < 4; ++d) {
-                    *(unsigned*)&Kt[l][8 * j + 2 * d][tc] = __builtin_amdgcn_perm(u1[d], u0[d], 0x05040100u);
-                    *(unsigned*)&Kt[l][8 * j + 2 * d + 1][tc] = __builtin_amdgcn_perm(u1[d], u0[d], 0x07060302u);
-                }
-            }
         }
         if (w == 0) {
             if (lane >= m) { ng = 0.f; nbt = 0.f; }
@@ -386,10 +420,14 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
         __syncthreads();
         if (t0 + C < len) fetch(t0 + C);
         if (tid == 0) kbad[par ^ 1] = C;
-        // A and P, the 16 x 16 blocks on and below the diagonal, as their transposes: a lane then holds what it will read, [row n][4 q ..]
-        for (int e = w; e < BLOCKS; e += NW) {
-            int bi = 0, bj = e;
-            while (bj > bi) { bj -= bi + 1; ++bi; }
+        // A and P, the 16 x 16 blocks on and below the diagonal, as their transposes: a lane then holds what it will read, [row n][4 q ..].
+        // The diagonal ones first: then one wave inverts those of I + A while the others see to the rest.
+        auto blocks = [&](int e) {
+            int bi = e, bj = e;
+            if (e >= CB) {
+                bi = 1; bj = e - CB;
+                while (bj >= bi) { bj -= bi; ++bi; }
+            }
             f32x4 xa = {0.f, 0.f, 0.f, 0.f}, xp = xa;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -426,44 +464,44 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
                 for (int l = 0; l < 3; ++l) Af[bi * bi / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
             }
-            if constexpr (MOVE) continue;
+            if constexpr (MOVE) return;
             uint4 f[PL];
             gd_split(xp, f, 0);
 #pragma unroll
             for (int l = 0; l < PL; ++l) Pf[(bi + 1) * (bi + 1) / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
-        }
+        };
+        if (w < BLOCKS) blocks(w);
         __syncthreads();
-        // inverses of the diagonal blocks of I + A: lane = column, forward substitution, in place
-        for (int bl = w; bl < CB; bl += NW) {
+        if (w == 0) {
+            // lane (q, n): column n of block q, forward substitution, in place
             float t[16];
+            float(*D)[20] = Ad[CB == 4 ? q : q & 1];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 float s = i == n ? 1.f : 0.f;
 #pragma unroll
-                for (int j = 0; j < i; ++j) s = __builtin_fmaf(Ad[bl][i][j], t[j], s);
+                for (int j = 0; j < i; ++j) s = __builtin_fmaf(D[i][j], t[j], s);
                 t[i] = s;
             }
-            if (lane < 16)
+            if (q < CB)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) Ad[bl][i][lane] = t[i];
-        }
-        // x = K S, y = Q S
-        f32x4 x[CB], y[CB];
-        {
-            uint4 sl[NC][3];
+                for (int i = 0; i < 16; ++i) D[i][n] = t[i];
+        } else
+            for (int e = NW + w - 1; e < BLOCKS; e += NW - 1) blocks(e);
+        // x = K S
+        f32x4 x[CB];
+        uint4 sl[NC][3];
 #pragma unroll
-            for (int c = 0; c < NB; ++c) gd_split(S[c], sl[c / 2], c & 1);
+        for (int c = 0; c < NB; ++c) gd_split(S[c], sl[c / 2], c & 1);
 #pragma unroll
-            for (int bl = 0; bl < CB; ++bl) {
-                x[bl] = (f32x4){0.f, 0.f, 0.f, 0.f}; y[bl] = x[bl];
+        for (int bl = 0; bl < CB; ++bl) {
+            x[bl] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    uint4 kf[L], qf[L];
+            for (int c = 0; c < NC; ++c) {
+                uint4 kf[L];
 #pragma unroll
-                    for (int l = 0; l < L; ++l) { kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q]; if constexpr (!MOVE) qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q]; }
-                    x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
-                    if constexpr (!MOVE) y[bl] = gd_mul<WIDE ? 2 : 1>(qf, sl[c], y[bl]);
-                }
+                for (int l = 0; l < L; ++l) kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q];
+                x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
             }
         }
         __syncthreads();
@@ -477,8 +515,12 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             { const int z = __shfl_xor(bad, 16); bad = z < bad ? z : bad; }
             { const int z = __shfl_xor(bad, 32); bad = z < bad ? z : bad; }
         }
-        uint4 ul[CC][3], wl[CC][3];
-        f32x4 o[CB];
+        const bool hurt = __any(bad < C);
+        const float end = eg[C - 1];
+        const auto ro = gd_buffer(a.out, ob + (long)t0 * a.os[1], (m - 1) * a.os[1] + a.Dv, E);
+        uint4 ul[CC][3], wl[3];
+#pragma unroll
+        for (int c = 0; c < NB; ++c) S[c] *= end;
 #pragma unroll
         for (int bl = 0; bl < CB; ++bl) {
             const float4 be = *(const float4*)&bt[16 * bl + 4 * q], e4 = *(const float4*)&eg[16 * bl + 4 * q], f4 = *(const float4*)&ee[16 * bl + 4 * q];
@@ -503,53 +545,54 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             u = mfma16(t.x, z[0], u); u = mfma16(t.y, z[1], u); u = mfma16(t.z, z[2], u); u = mfma16(t.w, z[3], u);
             gd_split(u, ul[bl / 2], bl & 1);
             if constexpr (!MOVE) {
-                o[bl][0] = a.scale * e4.x * y[bl][0]; o[bl][1] = a.scale * e4.y * y[bl][1]; o[bl][2] = a.scale * e4.z * y[bl][2]; o[bl][3] = a.scale * e4.w * y[bl][3];
+                // O's transpose: frame n, columns 4 q ..
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    uint4 qf[L];
+#pragma unroll
+                    for (int l = 0; l < L; ++l) qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q];
+                    o = gd_mul_t<WIDE ? 2 : 1>(qf, sl[c], o);
+                }
+                o *= a.scale * eg[16 * bl + n];
 #pragma unroll
                 for (int c = 0; c < (bl + 1) / 2; ++c) {
                     uint4 f[PL];
 #pragma unroll
                     for (int l = 0; l < PL; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
-                    o[bl] = gd_mul<PL - 1>(f, ul[c], o[bl]);
+                    o = gd_mul_t<PL - 1>(f, ul[c], o);
                 }
                 if (!(bl & 1)) {
                     uint2 f[PL];
 #pragma unroll
                     for (int l = 0; l < PL; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
-                    o[bl] = gd_mul16(f, ul[bl / 2], o[bl]);
+                    o = gd_mul16_t(f, ul[bl / 2], o);
                 }
+                if (hurt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (16 * bl + n >= __shfl(bad, 4 * q + i)) o[i] = gd_nan();
+                gd_put<T>(ro, ooff + 16 * bl * ostep, o, a.Dv - ocol, a.even);
             }
             u[0] *= f4.x; u[1] *= f4.y; u[2] *= f4.z; u[3] *= f4.w;
-            gd_split(u, wl[bl / 2], bl & 1);
+            gd_split(u, wl, bl & 1);
+            if (bl & 1)
+#pragma unroll
+                for (int c = 0; c < NB; ++c) {
+                    uint4 f[L];
+#pragma unroll
+                    for (int l = 0; l < L; ++l) {
+                        const unsigned short* p = &Kr[l][16 * (bl - 1) + 4 * q + (n >> 2)][32 * (c >> 1) + 8 * (n & 3) + 4 * (c & 1)];
+                        const uint2 f0 = gd_column(p), f1 = gd_column(p + 16 * LDK);
+                        f[l] = make_uint4(f0.x, f0.y, f1.x, f1.y);
+                    }
+                    S[c] = gd_mul<2>(f, wl, S[c]);
+                }
         }
-        const float end = eg[C - 1];
-#pragma unroll
-        for (int c = 0; c < NB; ++c) {
-            S[c] *= end;
-#pragma unroll
-            for (int k2 = 0; k2 < CC; ++k2) {
-                uint4 f[L];
-#pragma unroll
-                for (int l = 0; l < L; ++l) f[l] = *(const uint4*)&Kt[l][16 * c + n][32 * k2 + 8 * q];
-                S[c] = gd_mul<2>(f, wl[k2], S[c]);
-            }
-        }
-        if (__any(bad < C)) {
+        if (hurt && bad < C) {
             const float z = gd_nan();
-            if (bad < C)
 #pragma unroll
-                for (int c = 0; c < NB; ++c) S[c] = (f32x4){z, z, z, z};
-#pragma unroll
-            for (int bl = 0; bl < CB; ++bl)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (16 * bl + 4 * q + i >= bad) o[bl][i] = z;
-        }
-        if constexpr (!MOVE) {
-            const auto ro = gd_buffer(a.out, ob + (long)t0 * a.os[1], (m - 1) * a.os[1] + a.Dv, E);
-#pragma unroll
-            for (int bl = 0; bl < CB; ++bl)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) gd_put<T>(ro, ooff + (16 * bl + i) * ostep, o[bl][i]);
+            for (int c = 0; c < NB; ++c) S[c] = (f32x4){z, z, z, z};
         }
     }
     float* to = MOVE ? (eye ? a.moves + ((long)sg * heads + head) * a.Dk * a.Dk + col : a.starts + (long)(sg + 1) * heads * a.Dk * a.Dv + sb)

@@ -77,7 +77,7 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
         a.gs[i] = x.g_stride[i]; a.bs[i] = x.beta_stride[i]; a.os[i] = x.out_stride[i];
     }
     a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale; a.gate = x.gate_dtype;
-    a.segments = 1; a.seg = 0; a.starts = a.moves = nullptr; a.whole = 0; a.strips = 0;
+    a.segments = 1; a.seg = 0; a.starts = a.moves = nullptr; a.whole = a.even = 0; a.strips = 0;
     return DPDF_OK;
 }
 
@@ -171,6 +171,8 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
     a.whole = a.Dk % 8 == 0;
     for (const void* p : {a.q, a.k}) a.whole &= op_aligned(p, 4);
     for (const long* s : {a.qs, a.ks}) for (int i = 0; i < 3; ++i) a.whole &= s[i] * e % 4 == 0;
+    a.even = a.Dv % 4 == 0 && op_aligned(a.out, 4);
+    for (int i = 0; i < 3; ++i) a.even &= a.os[i] * e % 4 == 0;
     OpDevice dev(device);
     HIP_TRY(dev.err);
     const long heads = (long)args->batch * a.Hv, chunk = gd_chunk(args->dtype);
