@@ -13,6 +13,7 @@ struct W4Args {
     const void* bias;                             // [N], null: none
     void* y; long ys;                             // [M][N], row stride in elements
     int M, K, N, group;
+    unsigned tiles;                               // of 16 NT outputs
 };
 
 // Sixteen outputs at a time on the matrix units: x is the left operand (its rows the tile's rows, so that one row costs what sixteen do: the
@@ -23,132 +24,254 @@ struct W4Args {
 // Nibble t and t + 4 of a word come out together, so x is brought into the order 0 4 1 5 2 6 3 7.  fp32 rows go in as three bf16 limbs
 // (exact, see gru_limb.h), three products each.
 //
-// A workgroup is 16 NT outputs; its waves take every NW-th block of 128 inputs, their sums meet in LDS in a fixed order.  Lane (q, n) reads the
-// codes of output n: R words at a stretch, 32 R / 8 inputs.. of each run of 32 R inputs, so that a product's 32 inputs lie in one group
-// whatever its size: R = 4 where 128 divides the group, 2 where 64 does, else 1.
+// A workgroup is 16 NT outputs; each wave takes a run of blocks of 128 inputs, two blocks in flight, and the waves' sums meet in LDS in a fixed
+// order.  Lane (q, n) reads 16 bytes of output n's codes; the words then change places over q (four lane swaps), so that a product's 32 inputs are
+// 32 in a row: one group whatever its size, and x is read 64 bytes of a row at a time.  R such products are of one group: 4 where 128
+// divides the group, 2 where 64 does, else 1.  Scales and zeros are read for four blocks at once, those of block q by lane (q, n), and go through
+// LDS as fp32: read block by block, 2 bytes of 16 rows at a time, they cost more than the codes (8192 x 32768: 25 of 72 us).
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ unsigned w4_load4(const unsigned char* p) { unsigned v; __builtin_memcpy(&v, p, 4); return v; }
 
 template <typename T> struct W4X;                 // eight inputs of a row as a left operand: LIMBS fragments
 template <> struct W4X<__hip_bfloat16> { enum { LIMBS = 1 }; };
 template <> struct W4X<__half> { enum { LIMBS = 1 }; };
 template <> struct W4X<float> { enum { LIMBS = 3 }; };
 
-template <typename T> __device__ __forceinline__ uint4 w4_weights(unsigned w) {
-    uint4 r;
-    if constexpr (__is_same(T, __half)) {
-        r.x = ((w << 6) & 0x03c003c0u) | 0x4c004c00u; r.y = ((w << 2) & 0x03c003c0u) | 0x4c004c00u;
-        r.z = ((w >> 2) & 0x03c003c0u) | 0x4c004c00u; r.w = ((w >> 6) & 0x03c003c0u) | 0x4c004c00u;
-    } else {
-        r.x = ((w << 3) & 0x00780078u) | 0x41804180u; r.y = ((w >> 1) & 0x00780078u) | 0x41804180u;
-        r.z = ((w >> 5) & 0x00780078u) | 0x41804180u; r.w = ((w >> 9) & 0x00780078u) | 0x41804180u;
-    }
-    return r;
+// the eight weights of a word; mask and base (w4_mask, w4_base) come in registers of which one instruction can read both
+template <typename T> __device__ __forceinline__ unsigned w4_mask() { unsigned m = __is_same(T, __half) ? 0x03c003c0u : 0x00780078u; asm("" : "+v"(m)); return m; }
+template <typename T> __device__ __forceinline__ unsigned w4_base() { unsigned b = __is_same(T, __half) ? 0x4c004c00u : 0x41804180u; asm("" : "+s"(b)); return b; }
+template <typename T> __device__ __forceinline__ uint4 w4_weights(unsigned w, unsigned mask, unsigned base) {
+    if constexpr (__is_same(T, __half)) return make_uint4(((w << 6) & mask) | base, ((w << 2) & mask) | base, ((w >> 2) & mask) | base, ((w >> 6) & mask) | base);
+    else return make_uint4(((w << 3) & mask) | base, ((w >> 1) & mask) | base, ((w >> 5) & mask) | base, ((w >> 9) & mask) | base);
 }
 template <typename T> __device__ __forceinline__ unsigned w4_one() { return __is_same(T, __half) ? 0x3c003c00u : 0x3f803f80u; }
 template <typename T> __device__ __forceinline__ f32x4 w4_mfma(const uint4& a, const uint4& b, f32x4 c) {
     if constexpr (__is_same(T, __half)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
     else return mfma_bf16(a, b, c);
 }
-// eight consecutive inputs from index i of a row that ends at `end`
-template <typename T> __device__ __forceinline__ void w4_inputs(const void* x, long i, int left, uint4 (&f)[W4X<T>::LIMBS]) {
+// eight inputs in the codes' order, as limbs
+template <typename T> struct W4Eight { T v[8]; };
+template <typename T> __device__ __forceinline__ void w4_limbs(const W4Eight<T>& x, uint4 (&f)[W4X<T>::LIMBS]) {
     if constexpr (sizeof(T) == 2) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (left >= 8) __builtin_memcpy(&v, (const T*)x + i, 16);
-        else if (left > 0) {
-            unsigned short h[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = e < left ? ((const unsigned short*)x)[i + e] : 0;
-            v = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-        }
+        const uint4 v = __builtin_bit_cast(uint4, x);
         f[0] = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
                           __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
     } else {
-        float h[8];
-        if (left >= 8) __builtin_memcpy(h, (const float*)x + i, 32);
-        else
-#pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = e < left ? ((const float*)x)[i + e] : 0.f;
+        const float* h = x.v;
         uint2 a0, a1, a2, b0, b1, b2;
         split3(make_float4(h[0], h[4], h[1], h[5]), a0, a1, a2);
         split3(make_float4(h[2], h[6], h[3], h[7]), b0, b1, b2);
         f[0] = make_uint4(a0.x, a0.y, b0.x, b0.y); f[1] = make_uint4(a1.x, a1.y, b1.x, b1.y); f[2] = make_uint4(a2.x, a2.y, b2.x, b2.y);
     }
 }
+// rows of 16 lanes: the upper two of a with the lower two of b; the odd ones of a with the even ones of b
+__device__ __forceinline__ void w4_swap32(unsigned& a, unsigned& b) { const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false); a = r[0]; b = r[1]; }
+__device__ __forceinline__ void w4_swap16(unsigned& a, unsigned& b) { const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false); a = r[0]; b = r[1]; }
+
+constexpr int W4_WAVES = 8, W4_AHEAD = 2;        // waves of a workgroup at most; blocks of codes and inputs on their way
+// a block of 128 inputs as it is loaded
+template <int NT> struct W4Codes { gd_u4 v[NT]; };
+template <typename T> struct W4Inputs { W4Eight<T> v[4]; };
 
 template <typename T, typename G, int R, int NT>
-__global__ __launch_bounds__(512) void w4_matvec_kernel(W4Args a) {
-    constexpr int L = W4X<T>::LIMBS, SUB = 4 / R;       // groups that a block of 128 inputs is cut into
-    __shared__ float red[8][NT][16][17];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6, n = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16;
-    const bool row = m0 + n < a.M;                      // lane n of the left operand is row n of the tile
-    const long xi = (long)(m0 + n) * a.xs;
+__global__ __launch_bounds__(64 * W4_WAVES) void w4_matvec_kernel(W4Args a) {
+    constexpr int L = W4X<T>::LIMBS, SUB = 4 / R;       // SUB: groups that a block is cut into
+    typedef float2 Scales[4 * SUB][16 * NT];            // of four blocks: scale, -16 - zero
+    typedef float Sums[NT][16][17];
+    constexpr int ROOM = sizeof(Scales) > sizeof(Sums) ? sizeof(Scales) : sizeof(Sums);
+    __shared__ __attribute__((aligned(16))) unsigned char room[W4_WAVES][ROOM];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6, n = lane & 15, q = lane >> 4;
+    // Row tiles of the same outputs follow each other on one XCD, whose L2 then holds the codes: workgroups go to the eight XCDs in turn.
+    unsigned tile = blockIdx.x, mt = 0;
+    if (a.tiles != gridDim.x) {
+        const unsigned rows = gridDim.x / a.tiles, whole = a.tiles & ~7u, width = tile < whole * rows ? 8 : a.tiles & 7, from = tile < whole * rows ? tile / (8 * rows) * 8 : whole;
+        const unsigned r = tile - from * rows;
+        mt = r / width; tile = from + r % width;
+    }
+    const long n0 = (long)tile * 16 * NT;
+    const int m0 = mt * 16;
+    const bool zeros = a.zeros;
+    const T* xrow = (const T*)a.x + (long)(m0 + n < a.M ? m0 + n : a.M - 1) * a.xs;      // a tile's surplus rows and outputs are the last one again
     f32x4 y[NT];
-    long crow[NT], srow[NT], zrow[NT];
+    const unsigned char *crow[NT], *zrow[NT];
+    const G* srow[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        y[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        const int o = n0 + 16 * t + n < a.N ? n0 + 16 * t + n : a.N - 1;      // a tile's surplus outputs are the last one again
-        crow[t] = (long)o * a.cs; srow[t] = (long)o * a.ss; zrow[t] = (long)o * a.zs;
+        const long o = n0 + 16 * t + n < a.N ? n0 + 16 * t + n : a.N - 1;
+        crow[t] = a.codes + o * a.cs; srow[t] = (const G*)a.scales + o * a.ss;
+        zrow[t] = zeros ? a.zeros + o * a.zs : (const unsigned char*)srow[t];      // where there are none, bytes of the scales: read without a branch, not used
+        const float first = a.bias && w == 0 ? gd_load<T>(a.bias, o) : 0.f;      // the bias goes into the first wave's sums
+        y[t] = (f32x4){first, first, first, first};
     }
-    const int bytes = (a.K + 1) >> 1;
-    for (int kb = 128 * w; kb < a.K; kb += 128 * nw) {
+    const unsigned per32 = (unsigned)a.group / 32, mask = w4_mask<T>(), base = w4_base<T>();
+    Scales& sc = *(Scales*)room[w];
+    auto put = [&](const G (&s)[NT][SUB], const unsigned char (&z)[NT][SUB]) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) {
-            const int k0 = kb + 32 * R * s, k = k0 + 8 * R * q;
-            if (k0 >= a.K) break;
-            unsigned c[NT][R];
-            float sc[NT], zr[NT];
-            const int g = k0 / a.group;
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const unsigned char* p = a.codes + crow[t] + (k >> 1);
-                if (k + 8 * R <= a.K) __builtin_memcpy(c[t], p, 4 * R);
-                else
+            for (int u = 0; u < SUB; ++u) sc[SUB * q + u][16 * t + n] = make_float2(gd_load<G>(&s[t][u], 0), zeros ? -16.f - (float)z[t][u] : -24.f);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    // one block, the j-th of the four whose scales are in LDS
+    auto add = [&](const W4Codes<NT>& codes, const W4Inputs<T>& x, int j) {
+        unsigned c[NT][4];
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        c[t][r] = 0;
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if ((k >> 1) + 4 * r + e < bytes) c[t][r] |= (unsigned)p[4 * r + e] << (8 * e);
-                    }
-                sc[t] = gd_load<G>(a.scales, srow[t] + g);
-                zr[t] = a.zeros ? (float)a.zeros[zrow[t] + g] : 8.f;
-            }
+            for (int r = 0; r < 4; ++r) c[t][r] = codes.v[t][r];
+            w4_swap32(c[t][0], c[t][2]); w4_swap32(c[t][1], c[t][3]); w4_swap16(c[t][0], c[t][1]); w4_swap16(c[t][2], c[t][3]);
+        }
+        const unsigned o1 = w4_one<T>();
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
             f32x4 acc[NT], one = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < NT; ++t) acc[t] = one;
-            const unsigned o1 = w4_one<T>();
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
+            for (int r = R * u; r < R * (u + 1); ++r) {
                 uint4 f[L];
-                w4_inputs<T>(a.x, xi + k + 8 * r, row ? a.K - (k + 8 * r) : 0, f);
+                w4_limbs<T>(x.v[r], f);
 #pragma unroll
-                for (int l = L - 1; l >= 0; --l) {
-                    one = w4_mfma<T>(f[l], make_uint4(o1, o1, o1, o1), one);
+                for (int l = L - 1; l >= 0; --l) one = w4_mfma<T>(f[l], make_uint4(o1, o1, o1, o1), one);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) acc[t] = w4_mfma<T>(f[l], w4_weights<T>(c[t][r]), acc[t]);
+                for (int t = 0; t < NT; ++t) {
+                    const uint4 wt = w4_weights<T>(c[t][r], mask, base);
+#pragma unroll
+                    for (int l = L - 1; l >= 0; --l) acc[t] = w4_mfma<T>(f[l], wt, acc[t]);
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t) {
+                const float2 s = sc[SUB * j + u][16 * t + n];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[t][i] = __builtin_fmaf(sc[t], __builtin_fmaf(-16.f - zr[t], one[i], acc[t][i]), y[t][i]);
+                for (int i = 0; i < 4; ++i) y[t][i] = __builtin_fmaf(s.x, __builtin_fmaf(s.y, one[i], acc[t][i]), y[t][i]);
+            }
+        }
+    };
+    // the last wave takes what is left of the inputs, and nothing else where the others have no more to do for it
+    const int blocks = a.K >> 7, left = a.K & 127, alone = left && nw > 1 && (blocks + nw - 2) / (nw - 1) == (blocks + nw - 1) / nw;
+    const int per = (blocks + nw - 1) / nw, first = w * per, end = alone && w == nw - 1 ? 0 : blocks < first + per ? blocks : first + per;
+    if (first < end) {
+        // this lane's group in the next four blocks: that of the first 32 inputs of block q
+        unsigned g = 4 * (unsigned)(first + q) / per32, in = 4 * (unsigned)(first + q) - g * per32;
+        const unsigned dg = 16 / per32, din = 16 - dg * per32, top = 4 * (unsigned)(blocks - 1) / per32, most = ((unsigned)a.K - 1) / (unsigned)a.group;
+        auto scales = [&](G (&s)[NT][SUB], unsigned char (&z)[NT][SUB]) {
+            const unsigned g0 = g < top ? g : top;                 // behind the last block: read, not used
+            if (SUB == 1 || per32 == R)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) { __builtin_memcpy(s[t], srow[t] + g0, SUB * sizeof(G)); __builtin_memcpy(z[t], zrow[t] + g0, SUB); }
+            else
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    const unsigned g1 = g0 + (in + R * u >= per32), gu = g1 < most ? g1 : most;        // a group is longer than half a block: one border at most
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) { s[t][u] = srow[t][gu]; z[t][u] = zrow[t][gu]; }
+                }
+            g += dg; in += din;
+            if (in >= per32) { in -= per32; ++g; }
+        };
+        auto codes = [&](int i, W4Codes<NT>& c) {
+            const int at = i < end ? i : end - 1;                  // behind the last block: read, not used
+#pragma unroll
+            for (int t = 0; t < NT; ++t) __builtin_memcpy(&c.v[t], crow[t] + 64L * at + 16 * q, 16);
+        };
+        auto inputs = [&](int i, W4Inputs<T>& x) {
+            const int at = i < end ? i : end - 1;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) __builtin_memcpy(&x.v[r], xrow + 128L * at + 32 * r + 8 * q, sizeof(x.v[r]));
+        };
+        G s[NT][SUB];
+        unsigned char z[NT][SUB];
+        W4Codes<NT> c[W4_AHEAD];
+        W4Inputs<T> x[W4_AHEAD];
+        scales(s, z);
+#pragma unroll
+        for (int j = 0; j < W4_AHEAD; ++j) {
+            codes(first + j, c[j]);
+            inputs(first + j, x[j]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        int i = first;
+        for (; i + 4 < end; i += 4) {
+            put(s, z);
+            scales(s, z);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                add(c[j % W4_AHEAD], x[j % W4_AHEAD], j);
+                __builtin_amdgcn_sched_barrier(0);                 // the compiler would put the loads off to the end, behind all four blocks
+                codes(i + j + W4_AHEAD, c[j % W4_AHEAD]);
+                inputs(i + j + W4_AHEAD, x[j % W4_AHEAD]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        put(s, z);                                                 // one to four blocks, nothing to load behind them
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i + j >= end) break;
+            add(c[j % W4_AHEAD], x[j % W4_AHEAD], j);
+            if (j + W4_AHEAD < 4) {
+                codes(i + j + W4_AHEAD, c[j % W4_AHEAD]);
+                inputs(i + j + W4_AHEAD, x[j % W4_AHEAD]);
+            }
         }
     }
+    if (w == nw - 1 && left) {
+        const int k0 = a.K - left, last = (a.K - 1) >> 1;
+        unsigned char v[NT][16], z[NT][SUB];
+        G s[NT][SUB];
+        T xv[32];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int p = (k0 >> 1) + 16 * q + e;
+                v[t][e] = crow[t][p < last ? p : last];            // behind the end any code will do, x is 0 there
+            }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const int i = k0 + (e & ~7) * 4 + 8 * q + (e & 7);
+            xv[e] = xrow[i < a.K ? i : a.K - 1];
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) {
+            const int k = k0 + 32 * R * u, g = (k < a.K ? k : a.K - 1) / a.group;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) { s[t][u] = srow[t][g]; z[t][u] = zrow[t][g]; }
+        }
+        __builtin_amdgcn_sched_barrier(0);                         // all of the loads before the first use of one
+        W4Codes<NT> c;
+        W4Inputs<T> x;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c.v[t][r] = v[t][4 * r] | v[t][4 * r + 1] << 8 | v[t][4 * r + 2] << 16 | (unsigned)v[t][4 * r + 3] << 24;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+                if (k0 + 32 * R * u >= a.K) s[t][u] = (G)0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x.v[e / 8].v[e & 7] = k0 + (e & ~7) * 4 + 8 * q + (e & 7) < a.K ? xv[e] : (T)0.f;
+        put(s, z);
+        add(c, x, 0);
+    }
+    __syncthreads();
+    Sums& mine = *(Sums*)room[w];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) red[w][t][4 * q + i][n] = y[t][i];
+        for (int i = 0; i < 4; ++i) mine[t][4 * q + i][n] = y[t][i];
     __syncthreads();
     for (int e = threadIdx.x; e < NT * 256; e += blockDim.x) {
-        const int t = e >> 8, m = (e >> 4) & 15, c = e & 15, o = n0 + 16 * t + c;
+        const int t = e >> 8, m = (e >> 4) & 15, c = e & 15;
+        const long o = n0 + 16 * t + c;
         if (m0 + m >= a.M || o >= a.N) continue;
-        float v = red[0][t][m][c];
-        for (int i = 1; i < nw; ++i) v += red[i][t][m][c];
-        gd_store<T>(a.y, (long)(m0 + m) * a.ys + o, v + (a.bias ? gd_load<T>(a.bias, o) : 0.f));
+        float v[W4_WAVES];
+#pragma unroll
+        for (int i = 0; i < W4_WAVES; ++i) v[i] = (*(Sums*)room[i])[t][m][c];
+#pragma unroll
+        for (int i = 1; i < W4_WAVES; ++i) v[0] += i < nw ? v[i] : 0.f;
+        gd_store<T>(a.y, (long)(m0 + m) * a.ys + o, v[0]);
     }
 }
 
