@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import TYPE_CHECKING, Optional, Tuple
 
 from . import backend as _backend
@@ -42,27 +43,52 @@ class _W4QuantizeArgs(ctypes.Structure):
            ("zeros", _VP), ("zeros_pitch", _LONG)]
 
 
+# the same as bytes: packing them is several times faster than a Structure
+_GATED_DELTA, _W4_MATVEC = struct.Struct("@8i f 6P 18l 4P"), struct.Struct("@6i P l P l P l P l P P l")
+
+
 def _torch():
     import torch
     return torch
 
 
-_dtypes = None
+# A call's own time counts where a hop takes 3 us on the device: what it needs of torch and of the library is looked up once.
+class _Env:
+    def __init__(self):
+        torch = _torch()
+        self.torch, self.tensor, self.grad, self.empty = torch, torch.Tensor, torch.is_grad_enabled, torch.empty
+        self.dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+        self.f32, self.u8, self.i32 = torch.float32, torch.uint8, torch.int32
+        # the current stream's handle by device index, without a Stream object where torch offers that
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+        self.fns: dict = {}
+
+    def fn(self, name: str):
+        f = self.fns.get(name)
+        if f is None:
+            f = self.fns[name] = getattr(_backend.load_library(), name)
+        return f
+
+
+_the_env: Optional[_Env] = None
+
+
+def _env() -> _Env:
+    global _the_env
+    if _the_env is None:
+        _the_env = _Env()
+    return _the_env
 
 
 def _code(t, name: str) -> int:
-    global _dtypes
-    if _dtypes is None:
-        torch = _torch()
-        _dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
     try:
-        return _dtypes[t.dtype]
+        return _env().dtypes[t.dtype]
     except KeyError:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}") from None
 
 
 def _checked(device, shape, dtype, name: str, t):
-    """`t`, a tensor of this device, shape (None: any) and type whose last dimension is contiguous."""
+    """`t`, a tensor of this device, shape and type whose last dimension is contiguous."""
     torch = _torch()
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -79,53 +105,80 @@ def _checked(device, shape, dtype, name: str, t):
     return t
 
 
-def _call(fn, device, args, *workspace) -> None:
-    stream = _torch().cuda.current_stream(device).cuda_stream
-    _backend._check(getattr(_backend.load_library(), fn)(device.index, ctypes.addressof(args), *workspace, stream))
+def _strides(env, device, index, shape, dtype, name: str, t):
+    """The strides of `t` after `_checked`, whose messages it has where something does not fit."""
+    if isinstance(t, env.tensor) and t.get_device() == index >= 0 and t.shape == shape and t.dtype is dtype:
+        s = t.stride()
+        if (s[-1] == 1 or shape[-1] <= 1) and not (t.requires_grad and env.grad()):
+            return s
+    return _checked(device, shape, dtype, name, t).stride()
+
+
+def _gate_strides(env, device, index, shape, dtype, name: str, t):
+    """The same for a gate: it has one value per head, no contiguous dimension is asked of it."""
+    if isinstance(t, env.tensor) and t.get_device() == index >= 0 and t.shape == shape and t.dtype is dtype and not (t.requires_grad and env.grad()):
+        return t.stride()
+    return _checked(device, (*shape, 1), dtype, name, t[..., None] if isinstance(t, env.tensor) and t.dim() == 3 else t).stride()
+
+
+def _packed(fields, *values) -> bytes:
+    try:
+        return fields.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"a size or the scale is out of range: {e}") from None
+
+
+def _call(env, fn, index, args, *workspace) -> None:
+    rc = env.fn(fn)(index, args, *workspace, env.stream(index))
+    if rc:
+        _backend._check(rc)
 
 
 def _gated(fn, q, k, v, g, beta, state_in, state_out, lengths, active, scale, out):
-    torch = _torch()
+    env = _env()
     for name, t in (("q", q), ("v", v), ("g", g)):
-        if not isinstance(t, torch.Tensor):
+        if not isinstance(t, env.tensor):
             raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
-        if t.dim() != (3 if name == "g" else 4):
-            raise ValueError(f"{name} must have {3 if name == 'g' else 4} dimensions, got shape {list(t.shape)}")
-    dev, dt = q.device, q.dtype
-    B, T, Hk, Dk = q.shape
-    Hv, Dv = v.shape[2], v.shape[3]
+    if q.dim() != 4 or v.dim() != 4 or g.dim() != 3:
+        name, t, n = ("q", q, 4) if q.dim() != 4 else ("v", v, 4) if v.dim() != 4 else ("g", g, 3)
+        raise ValueError(f"{name} must have {n} dimensions, got shape {list(t.shape)}")
+    dev, index, dt, gt = q.device, q.get_device(), q.dtype, g.dtype
+    qshape = q.shape
+    B, T, Hk, Dk = qshape
+    _, _, Hv, Dv = v.shape
+    vshape = (B, T, Hv, Dv)
     code = _code(q, "q")
-    if g.dtype != torch.float32 and g.dtype != dt:
-        raise ValueError(f"g and beta must be float32 or {dt}, got {g.dtype}")
-    _checked(dev, (B, T, Hk, Dk), dt, "q", q)
-    _checked(dev, (B, T, Hk, Dk), dt, "k", k)
-    _checked(dev, (B, T, Hv, Dv), dt, "v", v)
-    # gates have one value per head: no contiguous dimension is asked of them
-    for name, t in (("g", g), ("beta", beta)):
-        _checked(dev, (B, T, Hv, 1), g.dtype, name, t[..., None] if isinstance(t, torch.Tensor) and t.dim() == 3 else t)
+    if gt is not env.f32 and gt is not dt:
+        raise ValueError(f"g and beta must be float32 or {dt}, got {gt}")
+    qs, ks, vs = _strides(env, dev, index, qshape, dt, "q", q), _strides(env, dev, index, qshape, dt, "k", k), _strides(env, dev, index, vshape, dt, "v", v)
+    gs, bs = _gate_strides(env, dev, index, (B, T, Hv), gt, "g", g), _gate_strides(env, dev, index, (B, T, Hv), gt, "beta", beta)
     for name, t in (("state", state_in), ("state_out", state_out)):
-        if t is not None and not _checked(dev, (B, Hv, Dk, Dv), torch.float32, name, t).is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+        if t is not None:
+            _strides(env, dev, index, (B, Hv, Dk, Dv), env.f32, name, t)
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+        if state_out is state_in:
+            break
     if lengths is not None:
-        _checked(dev, (B,), torch.int32, "lengths", lengths)
+        _strides(env, dev, index, (B,), env.i32, "lengths", lengths)
     if active is not None:
-        _checked(dev, (B,), torch.bool if getattr(active, "dtype", None) == torch.bool else torch.uint8, "active", active)
+        _strides(env, dev, index, (B,), env.torch.bool if getattr(active, "dtype", None) == env.torch.bool else env.u8, "active", active)
     if out is None:
         # what the call leaves unwritten is 0 in a result of its own
-        out = (torch.empty if lengths is None and active is None else torch.zeros)((B, T, Hv, Dv), device=dev, dtype=dt)
+        out = (env.empty if lengths is None and active is None else env.torch.zeros)(vshape, device=dev, dtype=dt)
+        os = out.stride()
     else:
-        _checked(dev, (B, T, Hv, Dv), dt, "out", out)
-    a = _GatedDeltaArgs(code, 0 if g.dtype == torch.float32 else code, B, T, Hk, Hv, Dk, Dv, 1.0 / math.sqrt(Dk) if scale is None else scale,
-                        q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
-                        q.stride()[:3], k.stride()[:3], v.stride()[:3], g.stride(), beta.stride(), out.stride()[:3],
-                        state_in.data_ptr() if state_in is not None else None, state_out.data_ptr() if state_out is not None else None,
-                        lengths.data_ptr() if lengths is not None else None, active.data_ptr() if active is not None else None)
+        os = _strides(env, dev, index, vshape, dt, "out", out)
+    a = _packed(_GATED_DELTA, code, 0 if gt is env.f32 else code, B, T, Hk, Hv, Dk, Dv, 1.0 / math.sqrt(Dk) if scale is None else float(scale),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(), out.data_ptr(),
+                *qs[:3], *ks[:3], *vs[:3], *gs[:3], *bs[:3], *os[:3], 0 if state_in is None else state_in.data_ptr(), 0 if state_out is None else state_out.data_ptr(),
+                0 if lengths is None else lengths.data_ptr(), 0 if active is None else active.data_ptr())
     if fn == "dpdf_gated_delta_step":
-        _call(fn, dev, a)
+        _call(env, fn, index, a)
     else:
-        need = _backend.load_library().dpdf_gated_delta_workspace(dev.index, ctypes.addressof(a))
-        room = torch.empty(need, device=dev, dtype=torch.uint8) if need else None        # given back to torch when the call is queued: this stream's next users follow it
-        _call(fn, dev, a, room.data_ptr() if need else None, need)
+        need = env.fn("dpdf_gated_delta_workspace")(index, a)
+        room = env.empty(need, device=dev, dtype=env.u8) if need else None        # given back to torch when the call is queued: this stream's next users follow it
+        _call(env, fn, index, a, room.data_ptr() if need else None, need)
     return out
 
 
@@ -167,37 +220,35 @@ def w4_matvec(x: "torch.Tensor", codes: "torch.Tensor", scales: "torch.Tensor", 
     x [M, K] (or [K]); codes [N, (K + 1) // 2] uint8, weight 2 i in the lower half of byte i; scales [N, ceil(K / group)] float32 or the type
     of x; zeros [N, ceil(K / group)] uint8, 0 .. 15 (8 everywhere if not given); bias [N] of the type of x; group a multiple of 32, the last
     one may be short.  `w4_quantize` makes codes, scales and zeros."""
-    torch = _torch()
+    env = _env()
     for name, t in (("x", x), ("codes", codes), ("scales", scales)):
-        if not isinstance(t, torch.Tensor):
+        if not isinstance(t, env.tensor):
             raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
     if x.dim() not in (1, 2) or codes.dim() != 2:
         raise ValueError(f"x must be [M, K] or [K] and codes [N, (K + 1) // 2], got {list(x.shape)} and {list(codes.shape)}")
-    x2 = x if x.dim() == 2 else x[None]
-    dev, dt = x.device, x.dtype
-    M, K = x2.shape
+    xshape, dev, index, dt, st = x.shape, x.device, x.get_device(), x.dtype, scales.dtype
+    M, K = xshape if len(xshape) == 2 else (1, xshape[0])
     N = codes.shape[0]
+    yshape = (M, N) if len(xshape) == 2 else (N,)
     code, group = _code(x, "x"), int(group)
     if group < 32 or group % 32:
         raise ValueError(f"group must be a multiple of 32, got {group}")
-    if scales.dtype != torch.float32 and scales.dtype != dt:
-        raise ValueError(f"scales must be float32 or {dt}, got {scales.dtype}")
+    if st is not env.f32 and st is not dt:
+        raise ValueError(f"scales must be float32 or {dt}, got {st}")
     groups = -(-K // group)
-    _checked(dev, (M, K), dt, "x", x2)
-    _checked(dev, (N, (K + 1) // 2), torch.uint8, "codes", codes)
-    _checked(dev, (N, groups), scales.dtype, "scales", scales)
-    if zeros is not None:
-        _checked(dev, (N, groups), torch.uint8, "zeros", zeros)
+    xs, cs = _strides(env, dev, index, xshape, dt, "x", x), _strides(env, dev, index, (N, (K + 1) // 2), env.u8, "codes", codes)
+    ss = _strides(env, dev, index, (N, groups), st, "scales", scales)
+    zs = _strides(env, dev, index, (N, groups), env.u8, "zeros", zeros) if zeros is not None else (0,)
     if bias is not None:
-        _checked(dev, (N,), dt, "bias", bias)
+        _strides(env, dev, index, (N,), dt, "bias", bias)
     if out is None:
-        out = torch.empty((M, N) if x.dim() == 2 else (N,), device=dev, dtype=dt)
+        out = env.empty(yshape, device=dev, dtype=dt)
+        ys = out.stride()
     else:
-        _checked(dev, (M, N) if x.dim() == 2 else (N,), dt, "out", out)
-    a = _W4MatvecArgs(code, 0 if scales.dtype == torch.float32 else code, M, K, N, group, x.data_ptr(), x2.stride(0), codes.data_ptr(), codes.stride(0),
-                      scales.data_ptr(), scales.stride(0), zeros.data_ptr() if zeros is not None else None, zeros.stride(0) if zeros is not None else 0,
-                      bias.data_ptr() if bias is not None else None, out.data_ptr(), out.stride(0) if out.dim() == 2 else N)
-    _call("dpdf_w4_matvec", dev, a)
+        ys = _strides(env, dev, index, yshape, dt, "out", out)
+    _call(env, "dpdf_w4_matvec", index,
+          _packed(_W4_MATVEC, code, 0 if st is env.f32 else code, M, K, N, group, x.data_ptr(), xs[0] if len(xshape) == 2 else K, codes.data_ptr(), cs[0],
+                  scales.data_ptr(), ss[0], 0 if zeros is None else zeros.data_ptr(), zs[0], 0 if bias is None else bias.data_ptr(), out.data_ptr(), ys[0] if len(xshape) == 2 else N))
     return out
 
 
@@ -221,5 +272,5 @@ def w4_quantize(weight: "torch.Tensor", *, group: int = 64, symmetric: bool = Fa
     zeros = None if symmetric else torch.empty((N, groups), device=dev, dtype=torch.uint8)
     a = _W4QuantizeArgs(code, K, N, group, weight.data_ptr(), weight.stride(0), codes.data_ptr(), pitch, scales.data_ptr(), groups,
                         zeros.data_ptr() if zeros is not None else None, groups)
-    _call("dpdf_w4_quantize", dev, a)
+    _call(_env(), "dpdf_w4_quantize", dev.index, ctypes.addressof(a))
     return codes, scales, zeros

@@ -97,6 +97,18 @@ def test_argument_structures_match_the_header(tmp_path):
         assert [int(n) for n in nums] == [ctypes.sizeof(cls)] + [getattr(cls, f[0]).offset for f in cls._fields_]
 
 
+@pytest.mark.parametrize("fields, cls", [(operators._GATED_DELTA, operators._GatedDeltaArgs), (operators._W4_MATVEC, operators._W4MatvecArgs)])
+def test_packed_arguments_are_the_structures(fields, cls):
+    flat = [n for n, t in cls._fields_ for _ in range(3 if t is operators._L3 else 1)]
+    a = cls.from_buffer_copy(fields.pack(*(i + 1 for i in range(len(flat)))))
+    got = []
+    for n, t in cls._fields_:
+        got += list(getattr(a, n)) if t is operators._L3 else [getattr(a, n)]
+    assert got == [i + 1 for i in range(len(flat))]
+    with pytest.raises(ValueError, match="out of range"):
+        operators._packed(fields, *(2 ** 40 for _ in flat))
+
+
 def test_operators_are_reachable_under_both_names():
     import dpdfnet.operators as alias
     assert alias is operators
