@@ -16,9 +16,10 @@ struct GatedDeltaArgs {
     const int* lengths;               // [B], null: T each
     const unsigned char* active;      // [B], null: all
     long qs[3], ks[3], vs[3], gs[3], bs[3], os[3];      // strides in elements: batch, frame, head
-    int T, Hk, Hv, Dk, Dv;
+    int B, T, Hk, Hv, Dk, Dv;
     int strips;                       // workgroups (clip) or waves (step) per head
     int gate;                         // type of g and beta: 0 fp32, 1 fp16, 2 bf16
+    int sorted;                       // clips: the longest first (batch: at most GD_RANKED)
     int whole, even;                  // clips: k and q can be read in pieces of eight values, out written in pieces of four
     int segments, seg;                // clips: how many pieces a clip is cut into, and their frames
     float* starts;                    // [segments][B Hv][Dk][Dv]: the states that segments 1 .. start with; before they are joined, what each adds
@@ -294,6 +295,31 @@ __device__ __forceinline__ uint2 gd_column(const unsigned short* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) gd_s4*)p));
 }
 
+// The clip that is `place`-th in a batch from long to short: thread i counts the clips before clip i, by chunks of 16 frames and number.  Workgroups
+// start in this order, so that no long clip begins when the others are done; the order has no part in the results.
+constexpr int GD_RANKED = 256;                             // clips of a batch that is put in order, the threads of the smaller workgroup
+__device__ __forceinline__ int gd_ranked(const GatedDeltaArgs& a, int place) {
+    __shared__ __attribute__((aligned(16))) unsigned keys[GD_RANKED];
+    __shared__ int found;
+    const int i = threadIdx.x;
+    unsigned mine = 0;
+    if (i < a.B) {
+        const int n = a.lengths[i];
+        mine = (n < 0 ? 0u : (unsigned)(n > a.T ? a.T : n) >> 4) << 8 | (255u - i);
+    }
+    if (i < GD_RANKED) keys[i] = mine;
+    __syncthreads();
+    int before = 0;
+#pragma unroll 8
+    for (int j = 0; j < GD_RANKED; j += 4) {
+        const uint4 k = *(const uint4*)&keys[j];
+        before += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+    }
+    if (i < a.B && before == place) found = i;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(found);
+}
+
 template <typename T, int DKP, int NW, int C, bool MOVE>
 __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDeltaArgs a) {
     constexpr int L = GdIn<T>::L, NB = DKP / 16, NC = DKP / 32, CB = C / 16, CC = C / 32, LDK = DKP + 8, E = sizeof(T);
@@ -311,8 +337,11 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
     const long unit = blockIdx.x / a.strips;               // (head, segment)
     const int sg = (int)(unit % a.segments);
-    const long head = unit / a.segments, heads = (long)(gridDim.x / a.strips) / a.segments;
-    const int b = (int)(head / a.Hv), h = (int)(head - (long)b * a.Hv), hk = h / (a.Hv / a.Hk);
+    long head = unit / a.segments;
+    const long heads = (long)(gridDim.x / a.strips) / a.segments;
+    int b = (int)(head / a.Hv);
+    const int h = (int)(head - (long)b * a.Hv), hk = h / (a.Hv / a.Hk);
+    if (!MOVE && a.sorted) { b = gd_ranked(a, b); head = (long)b * a.Hv + h; }
     int col = 16 * NW * (int)(blockIdx.x - unit * a.strips) + 16 * w + n;
     const int vcols = (a.Dv + 15) & ~15;
     const bool eye = MOVE && col >= vcols;                 // a column of the unit matrix: the same for a wave

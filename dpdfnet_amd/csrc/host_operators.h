@@ -76,8 +76,8 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
         a.qs[i] = x.q_stride[i]; a.ks[i] = x.k_stride[i]; a.vs[i] = x.v_stride[i];
         a.gs[i] = x.g_stride[i]; a.bs[i] = x.beta_stride[i]; a.os[i] = x.out_stride[i];
     }
-    a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale; a.gate = x.gate_dtype;
-    a.segments = 1; a.seg = 0; a.starts = a.moves = nullptr; a.whole = a.even = 0; a.strips = 0;
+    a.B = x.batch; a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale; a.gate = x.gate_dtype;
+    a.segments = 1; a.seg = 0; a.starts = a.moves = nullptr; a.whole = a.even = a.sorted = 0; a.strips = 0;
     return DPDF_OK;
 }
 
@@ -198,6 +198,12 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
             for (const OpSpan& o : other) if (op_meet(ws, o)) return set_err(DPDF_E_INVALID, "gated delta rule: the workspace overlaps a tensor");
             a.starts = (float*)workspace; a.moves = a.starts + (size_t)a.segments * heads * a.Dk * a.Dv;
         }
+    }
+    if (a.lengths && a.segments == 1 && a.B <= GD_RANKED && a.T < 1 << 25) {
+        int cus = 0;
+        HIP_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
+        // all of them start at once otherwise (256 clips of 334 to 1003 frames, 4 heads of 64 in bf16: 205 us in the batch's order, 178 us so)
+        a.sorted = heads * ((a.Dv + gd_columns(a) - 1) / gd_columns(a)) > (long)cus * gd_resident(a);
     }
     gd_type(args->dtype, [&](auto t) { gd_launch_clips<decltype(t)>(a, heads, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());

@@ -322,6 +322,27 @@ def test_ragged_clips_leave_the_rest_alone(lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B, T, lens", [(256, 40, "any"), (200, 70, "any"), (180, 33, "equal"), (257, 20, "any")])
+def test_many_clips_of_any_lengths(B, T, lens, dtype):
+    """More clips than start at once, whatever order they are started in."""
+    x = inputs(B, T, 2, 4, 16, 32, dtype, seed=B)
+    gen = torch.Generator().manual_seed(B)
+    n = torch.full((B,), 17) if lens == "equal" else torch.randint(-3, T + 4, (B,), generator=gen)
+    n = n.to(torch.int32)
+    out = torch.full((B, T, 4, 32), 5.0, dtype=dtype, device="cuda")
+    got, end = operators.gated_delta(*x, lengths=n.cuda(), out=out)
+    ref, rend = delta_rule(*x, lengths=n.clamp(0, T))
+    on = (torch.arange(T)[None] < n[:, None]).cuda()
+    assert bool((got[~on] == 5).all())
+    near(torch.where(on[..., None, None], got, 0), ref, tol(T, 16), HALF_STEP[dtype], TINY[dtype])
+    near(end, rend, tol(T, 16))
+    alone = [operators.gated_delta(*(t[b:b + 1] for t in x), lengths=n[b:b + 1].cuda()) for b in (0, 1, B - 1)]
+    for (o, e), b in zip(alone, (0, 1, B - 1)):
+        assert torch.equal(e[0], end[b]) and torch.equal(o[0][on[b]], got[b][on[b]])
+
+
+@pytest.mark.gpu
 def test_clips_without_a_frame():
     x = inputs(2, 4, 1, 1, 16, 16, F32)
     none = [t[:, :0] for t in x]
