@@ -517,20 +517,27 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 for (int i = 0; i < 16; ++i) D[i][n] = t[i];
         } else
             for (int e = NW + w - 1; e < BLOCKS; e += NW - 1) blocks(e);
-        // x = K S
-        f32x4 x[CB];
-        uint4 sl[NC][3];
+        // x = K S, o = the transpose of Q S: frame n, columns 4 q ..
+        f32x4 x[CB], o[MOVE ? 1 : CB];
+        {
+            uint4 sl[NC][3];
 #pragma unroll
-        for (int c = 0; c < NB; ++c) gd_split(S[c], sl[c / 2], c & 1);
+            for (int c = 0; c < NB; ++c) gd_split(S[c], sl[c / 2], c & 1);
 #pragma unroll
-        for (int bl = 0; bl < CB; ++bl) {
-            x[bl] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            for (int bl = 0; bl < CB; ++bl) {
+                x[bl] = (f32x4){0.f, 0.f, 0.f, 0.f};
+                if constexpr (!MOVE) o[bl] = x[bl];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                uint4 kf[L];
+                for (int c = 0; c < NC; ++c) {
+                    uint4 kf[L], qf[L];
 #pragma unroll
-                for (int l = 0; l < L; ++l) kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q];
-                x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
+                    for (int l = 0; l < L; ++l) {
+                        kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q];
+                        if constexpr (!MOVE) qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q];
+                    }
+                    x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
+                    if constexpr (!MOVE) o[bl] = gd_mul_t<WIDE ? 2 : 1>(qf, sl[c], o[bl]);
+                }
             }
         }
         __syncthreads();
@@ -574,34 +581,25 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             u = mfma16(t.x, z[0], u); u = mfma16(t.y, z[1], u); u = mfma16(t.z, z[2], u); u = mfma16(t.w, z[3], u);
             gd_split(u, ul[bl / 2], bl & 1);
             if constexpr (!MOVE) {
-                // O's transpose: frame n, columns 4 q ..
-                f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    uint4 qf[L];
-#pragma unroll
-                    for (int l = 0; l < L; ++l) qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q];
-                    o = gd_mul_t<WIDE ? 2 : 1>(qf, sl[c], o);
-                }
-                o *= a.scale * eg[16 * bl + n];
+                o[bl] *= a.scale * eg[16 * bl + n];
 #pragma unroll
                 for (int c = 0; c < (bl + 1) / 2; ++c) {
                     uint4 f[PL];
 #pragma unroll
                     for (int l = 0; l < PL; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
-                    o = gd_mul_t<PL - 1>(f, ul[c], o);
+                    o[bl] = gd_mul_t<PL - 1>(f, ul[c], o[bl]);
                 }
                 if (!(bl & 1)) {
                     uint2 f[PL];
 #pragma unroll
                     for (int l = 0; l < PL; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
-                    o = gd_mul16_t(f, ul[bl / 2], o);
+                    o[bl] = gd_mul16_t(f, ul[bl / 2], o[bl]);
                 }
                 if (hurt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (16 * bl + n >= __shfl(bad, 4 * q + i)) o[i] = gd_nan();
-                gd_put<T>(ro, ooff + 16 * bl * ostep, o, a.Dv - ocol, a.even);
+                        if (16 * bl + n >= __shfl(bad, 4 * q + i)) o[bl][i] = gd_nan();
+                gd_put<T>(ro, ooff + 16 * bl * ostep, o[bl], a.Dv - ocol, a.even);
             }
             u[0] *= f4.x; u[1] *= f4.y; u[2] *= f4.z; u[3] *= f4.w;
             gd_split(u, wl, bl & 1);
@@ -654,34 +652,41 @@ __global__ __launch_bounds__(4 * DKP) void gated_delta_join_kernel(GatedDeltaArg
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = cin && row + i < a.Dk ? a.starts[(long)s * step + sb + (long)(row + i) * a.Dv] : 0.f;
     };
-    auto matrix = [&](int s, float (&x)[NB][4]) {
+    const bool whole = a.Dk % 4 == 0;
+    auto matrix = [&](int s, f32x4 (&x)[NB]) {
+        if (whole)
 #pragma unroll
-        for (int c = 0; c < NB; ++c)
+            for (int c = 0; c < NB; ++c) x[c] = 16 * c + 4 * q < a.Dk ? *(const f32x4*)&mv[(long)s * mstep + 16 * c + 4 * q] : (f32x4){0.f, 0.f, 0.f, 0.f};
+        else
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[c][i] = 16 * c + 4 * q + i < a.Dk ? mv[(long)s * mstep + 16 * c + 4 * q + i] : 0.f;
+            for (int c = 0; c < NB; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[c][i] = 16 * c + 4 * q + i < a.Dk ? mv[(long)s * mstep + 16 * c + 4 * q + i] : 0.f;
     };
-    float x[4], nx[4], m[NB][4];
+    // segment s's matrix and the next one's addition are on their way while segment s - 1 is joined
+    float x[4], nx[4];
+    f32x4 m[NB];
     piece(1, x);
     if (a.segments > 2) { matrix(1, m); piece(2, nx); }
     for (int s = 1; s + 1 < a.segments; ++s) {
         *(float4*)&Sx[s & 1][n][row] = make_float4(x[0], x[1], x[2], x[3]);
         __syncthreads();
-        f32x4 y = {nx[0], nx[1], nx[2], nx[3]};
-        float cm[NB][4];
+        f32x4 y[4] = {{nx[0], nx[1], nx[2], nx[3]}}, cm[NB];      // four sums, so that the products need not wait for each other
 #pragma unroll
-        for (int c = 0; c < NB; ++c)
+        for (int c = 1; c < 4; ++c) y[c] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) cm[c][i] = m[c][i];
+        for (int c = 0; c < NB; ++c) cm[c] = m[c];
         if (s + 2 < a.segments) { matrix(s + 1, m); piece(s + 2, nx); }
 #pragma unroll
         for (int c = 0; c < NB; ++c) {
             const float4 v = *(const float4*)&Sx[s & 1][n][16 * c + 4 * q];
-            y = mfma16(cm[c][0], v.x, y); y = mfma16(cm[c][1], v.y, y); y = mfma16(cm[c][2], v.z, y); y = mfma16(cm[c][3], v.w, y);
+            y[0] = mfma16(cm[c][0], v.x, y[0]); y[1] = mfma16(cm[c][1], v.y, y[1]); y[2] = mfma16(cm[c][2], v.z, y[2]); y[3] = mfma16(cm[c][3], v.w, y[3]);
         }
+        y[0] += y[1]; y[2] += y[3]; y[0] += y[2];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] = row + i < a.Dk ? y[i] : 0.f;
-            if (cin && row + i < a.Dk) a.starts[(long)(s + 1) * step + sb + (long)(row + i) * a.Dv] = y[i];
+            x[i] = row + i < a.Dk ? y[0][i] : 0.f;
+            if (cin && row + i < a.Dk) a.starts[(long)(s + 1) * step + sb + (long)(row + i) * a.Dv] = y[0][i];
         }
     }
 }
