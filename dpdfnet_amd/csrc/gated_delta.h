@@ -20,7 +20,7 @@ struct GatedDeltaArgs {
     int strips;                       // workgroups (clip) or waves (step) per head
     int gate;                         // type of g and beta: 0 fp32, 1 fp16, 2 bf16
     int sorted;                       // clips: the longest first (batch: at most GD_RANKED)
-    int whole, even;                  // clips: k and q can be read in pieces of eight values, out written in pieces of four
+    int whole, even;                  // k and q can be read in pieces of eight values (hops: v in pieces of four too), out written in pieces of four
     int segments, seg;                // clips: how many pieces a clip is cut into, and their frames
     float* starts;                    // [segments][B Hv][Dk][Dv]: the states that segments 1 .. start with; before they are joined, what each adds
     float* moves;                     // [segments][B Hv][Dk][Dk]: segment i's effect on the state before it, i = 1 .. segments - 2
@@ -44,133 +44,9 @@ __device__ __forceinline__ float gd_gate(const void* p, long i, int type) {
 __device__ __forceinline__ bool gd_finite(float v) { return (__builtin_bit_cast(unsigned, v) & 0x7f800000u) != 0x7f800000u; }
 __device__ __forceinline__ float gd_nan() { return __builtin_bit_cast(float, 0x7fc00000u); }
 
-// ---------------------------------------------------------------------------------------------------------------------------------------
-// Hops: one wave = 32 columns of one head's state, all Dk rows of them in registers for the T hops of the call; lane (rg, cl) holds the
-// DKP / 8 rows rg * DKP / 8 + j of the columns 4 cl .. 4 cl + 3.  A hop needs S'^T k and S'^T q; with o = scale (S'^T q + (q.k) e) both are
-// sums over the OLD state, so that one butterfly over the eight row groups serves them, and no wave waits for another.
-// Bound: HBM, the state read once and written once.
-// ---------------------------------------------------------------------------------------------------------------------------------------
-template <typename T, int DKP, bool WHOLE>
-__global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) {
-    constexpr int R = DKP / 8;
-    const int lane = threadIdx.x, cl = lane & 7, rg = lane >> 3;
-    const long head = blockIdx.x / a.strips;
-    const int strip = (int)(blockIdx.x - head * a.strips);
-    const int b = (int)(head / a.Hv), h = (int)(head - (long)b * a.Hv), hk = h / (a.Hv / a.Hk);
-    if (a.active && !a.active[b]) return;
-    const int c0 = 32 * strip + 4 * cl, r0 = rg * R;
-    const long sbase = head * a.Dk * a.Dv;
-    float S[R][4];
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const int r = r0 + j;
-        const float* p = a.state_in + sbase + (long)r * a.Dv + c0;
-        if constexpr (WHOLE) {
-            const float4 s = *(const float4*)p;
-            S[j][0] = s.x; S[j][1] = s.y; S[j][2] = s.z; S[j][3] = s.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][i] = r < a.Dk && c0 + i < a.Dv ? p[i] : 0.f;
-        }
-    }
-    const long qb = (long)b * a.qs[0] + (long)hk * a.qs[2], kb = (long)b * a.ks[0] + (long)hk * a.ks[2];
-    const long vb = (long)b * a.vs[0] + (long)h * a.vs[2] + c0, ob = (long)b * a.os[0] + (long)h * a.os[2] + c0;
-    const long gb = (long)b * a.gs[0] + (long)h * a.gs[2], bb = (long)b * a.bs[0] + (long)h * a.bs[2];
-    for (int t = 0; t < a.T; ++t) {
-        float kr[R], qr[R], v[4];
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            const bool in = WHOLE || r0 + j < a.Dk;
-            kr[j] = in ? gd_load<T>(a.k, kb + t * a.ks[1] + r0 + j) : 0.f;
-            qr[j] = in ? gd_load<T>(a.q, qb + t * a.qs[1] + r0 + j) : 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = WHOLE || c0 + i < a.Dv ? gd_load<T>(a.v, vb + t * a.vs[1] + i) : 0.f;
-        const float alpha = __expf(gd_gate(a.g, gb + t * a.gs[1], a.gate)), beta = gd_gate(a.beta, bb + t * a.bs[1], a.gate);
-        float sk[4] = {0.f, 0.f, 0.f, 0.f}, sq[4] = {0.f, 0.f, 0.f, 0.f}, qk = 0.f;
-#pragma unroll
-        for (int j = 0; j < R; ++j) {
-            qk = __builtin_fmaf(qr[j], kr[j], qk);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                S[j][i] *= alpha;
-                sk[i] = __builtin_fmaf(kr[j], S[j][i], sk[i]);
-                sq[i] = __builtin_fmaf(qr[j], S[j][i], sq[i]);
-            }
-        }
-#pragma unroll
-        for (int m = 8; m < 64; m <<= 1) {
-            qk += __shfl_xor(qk, m);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { sk[i] += __shfl_xor(sk[i], m); sq[i] += __shfl_xor(sq[i], m); }
-        }
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[i] = beta * (v[i] - sk[i]);
-#pragma unroll
-        for (int j = 0; j < R; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) S[j][i] = __builtin_fmaf(kr[j], e[i], S[j][i]);
-        if (rg == 0)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (WHOLE || c0 + i < a.Dv) gd_store<T>(a.out, ob + t * a.os[1] + i, a.scale * __builtin_fmaf(qk, e[i], sq[i]));
-    }
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-        const int r = r0 + j;
-        float* p = a.state_out + sbase + (long)r * a.Dv + c0;
-        if constexpr (WHOLE) *(float4*)p = make_float4(S[j][0], S[j][1], S[j][2], S[j][3]);
-        else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r < a.Dk && c0 + i < a.Dv) p[i] = S[j][i];
-        }
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------------------------------
-// Clips: chunks of C frames.  With gamma = the running sum of g inside the chunk, d_ij = exp(gamma_i - gamma_j) and S the state before it,
-//     A_ij = beta_i d_ij k_i.k_j (j < i),   (I + A) u = beta (v - exp(gamma) (K S)),
-//     O = scale exp(gamma) (Q S) + P u,   P_ij = scale d_ij q_i.k_j (j <= i),   S <- exp(gamma_C) S + K^T (exp(gamma_C - gamma) u):
-// matrix products, and 16 dependent steps for the inverses of the 16 x 16 diagonal blocks of I + A where the definition has C.
-//
-// A workgroup is one head and 16 NW columns: wave w owns 16 columns of S, u and O in the matrix units' result layout (row 4 q + i, column n),
-// in which a result IS the next product's right operand -- K slot 8 q + 4 h + i of two 16-row blocks is row 4 q + i of block h -- so that
-// K S -> u -> P u, K^T u chain in registers, and the waves meet only over the chunk's K, Q, A and P in LDS, which are laid out in that order.
-//
-// Every fp32 operand goes in as bf16 limbs (split3 of gru_limb.h: exact), products of limbs whose indices add up to more than 2 (2^-24 of the
-// term) left out; bf16 values of k and q are one limb, fp16 two, fp32 three.  What only reaches the outputs of a 16-bit type (Q S, P u) takes two
-// limbs of either side, 2^-16 of a term against the 2^-8 and 2^-11 of the result's rounding; the state's path takes all.
-//
-// Where there are fewer heads than the chip holds workgroups, the frames are cut into segments.  A segment's effect on the state before it is
-// linear, S -> M S + N: MOVE runs a segment from S = 0 with its v (N) and from the unit matrix without (M, Dk columns more), no outputs;
-// gated_delta_join_kernel then walks the segments (N becomes the state that the next one starts with), and the segments run as
-// clips of their own.  About two and a half times the work, over `segments` times the workgroups.
-//
-// gamma and its differences are 64-bit: they are small differences of long sums.  A non-finite k, g or beta makes its head's outputs from its
-// frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all
-// frames of the chunk, so that such values are taken out of the operands first).
-// ---------------------------------------------------------------------------------------------------------------------------------------
-template <typename T> struct GdIn;
-template <> struct GdIn<__hip_bfloat16> { enum { L = 1 }; };
-template <> struct GdIn<__half> { enum { L = 2 }; };
-template <> struct GdIn<float> { enum { L = 3 }; };
-
-// the running sum over a wave's lanes
-__device__ __forceinline__ double gd_scan(double v) {
-#define GD_STEP_(ctrl, rows) { \
-        const unsigned long b = __builtin_bit_cast(unsigned long, v); \
-        const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, ctrl, rows, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), ctrl, rows, 0xf, false); \
-        v += __builtin_bit_cast(double, (unsigned long)hi << 32 | lo); }
-    GD_STEP_(0x111, 0xf) GD_STEP_(0x112, 0xf) GD_STEP_(0x114, 0xf) GD_STEP_(0x118, 0xf)      // row_shr 1, 2, 4, 8: inside 16 lanes
-    GD_STEP_(0x142, 0xa) GD_STEP_(0x143, 0xc)                                                // lane 15's sum to the next row, lane 31's to the upper half
-#undef GD_STEP_
-    return v;
-}
-// What a chunk reads and writes goes through buffer descriptors that end with its last frame: behind that, and at GD_OUT, loads give 0 and stores
-// do nothing, so that there is no branch around a load (behind one the compiler cannot count the loads in flight and waits for them), no
-// clamp and 32 bits of address.
+// What a hop or a chunk reads and writes goes through buffer descriptors that end with it: behind that, and at GD_OUT, loads give 0 and stores do
+// nothing, so that there is no branch around a load (behind one the compiler cannot count the loads in flight and waits for them), no clamp
+// and 32 bits of address.
 constexpr unsigned GD_OUT = 0x80000000u;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t gd_buffer(const void* base, long first, long count, int elem) {
     return __builtin_amdgcn_make_buffer_rsrc((void*)((const char*)base + first * elem), 0, (int)(count * elem), 0x00027000);
@@ -227,6 +103,141 @@ template <typename T> __device__ __forceinline__ void gd_put(__amdgpu_buffer_rsr
 #pragma unroll
             for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[i / 2] >> (16 * (i & 1))), r, i < left ? off + 2 * i : GD_OUT, 0, 0);
     }
+}
+// N bytes into registers
+template <int N> __device__ __forceinline__ void gd_piece(__amdgpu_buffer_rsrc_t r, unsigned off, void* to) {
+    if constexpr (N == 2) { const unsigned short v = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0); __builtin_memcpy(to, &v, 2); }
+    else if constexpr (N == 4) { const unsigned v = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0); __builtin_memcpy(to, &v, 4); }
+    else if constexpr (N == 8) { const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0); __builtin_memcpy(to, &v, 8); }
+    else { const gd_u4 v = __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0); __builtin_memcpy(to, &v, 16); }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------
+// Hops: one wave = 32 columns of one head's state, all Dk rows of them in registers for the T hops of the call; lane (rg, cl) holds the
+// DKP / 8 rows rg * DKP / 8 + j of the columns 4 cl .. 4 cl + 3.  A hop needs S'^T k and S'^T q; with o = scale (S'^T q + (q.k) e) both are
+// sums over the OLD state, so that one butterfly over the eight row groups serves them, and no wave waits for another.
+// Rows behind Dk are loaded as 0; a column behind Dv holds what comes next in memory, meets no other column and is not stored.
+// Bound: HBM, the state read once and written once (192 streams of 32 heads of 128 x 128, two hops: 162 us, 5.0 TB/s; a large copy does 5.1).
+// ---------------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int R> struct GdHop { T k[R], q[R], v[4]; float g, beta; };      // what a lane reads for a hop
+
+template <typename T, int DKP, bool WHOLE>
+__global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) {
+    constexpr int R = DKP / 8, E = sizeof(T);
+    const int lane = threadIdx.x, cl = lane & 7, rg = lane >> 3;
+    const unsigned head = blockIdx.x / (unsigned)a.strips, strip = blockIdx.x - head * a.strips, b = head / (unsigned)a.Hv, h = head - b * a.Hv, hk = h / (unsigned)(a.Hv / a.Hk);
+    if (a.active && !a.active[b]) return;
+    const int c0 = 32 * (int)strip + 4 * cl, r0 = rg * R;
+    const long sbase = (long)head * a.Dk * a.Dv;
+    const auto si = gd_buffer(a.state_in, sbase, (long)a.Dk * a.Dv, 4), so = gd_buffer(a.state_out, sbase, (long)a.Dk * a.Dv, 4);
+    f32x4 S[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+        S[j] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(si, r0 + j < a.Dk ? ((unsigned)(r0 + j) * a.Dv + c0) * 4 : GD_OUT, 0, 0));
+    const long qb = (long)b * a.qs[0] + (long)hk * a.qs[2], kb = (long)b * a.ks[0] + (long)hk * a.ks[2];
+    const long vb = (long)b * a.vs[0] + (long)h * a.vs[2], ob = (long)b * a.os[0] + (long)h * a.os[2];
+    const long gb = (long)b * a.gs[0] + (long)h * a.gs[2], bb = (long)b * a.bs[0] + (long)h * a.bs[2];
+    auto fetch = [&](int t) {
+        GdHop<T, R> x;
+        const auto rk = gd_buffer(a.k, kb + t * a.ks[1], a.Dk, E), rq = gd_buffer(a.q, qb + t * a.qs[1], a.Dk, E), rv = gd_buffer(a.v, vb + t * a.vs[1], a.Dv, E);
+        if constexpr (WHOLE) {
+            // rows in pieces of 4 bytes or more; one that begins inside Dk ends there
+            constexpr int P = R * E % 16 == 0 ? 16 : R * E % 8 == 0 ? 8 : 4;
+#pragma unroll
+            for (int e = 0; e < R * E / P; ++e) {
+                const unsigned o = r0 * E + P * e < (unsigned)(a.Dk * E) ? r0 * E + P * e : GD_OUT;
+                gd_piece<P>(rk, o, (char*)x.k + P * e); gd_piece<P>(rq, o, (char*)x.q + P * e);
+            }
+            gd_piece<4 * E>(rv, c0 * E, x.v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < R; ++j) {
+                const unsigned o = r0 + j < a.Dk ? (r0 + j) * E : GD_OUT;
+                gd_piece<E>(rk, o, &x.k[j]); gd_piece<E>(rq, o, &x.q[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) gd_piece<E>(rv, (c0 + i) * E, &x.v[i]);
+        }
+        x.g = gd_gate(a.g, gb + t * a.gs[1], a.gate); x.beta = gd_gate(a.beta, bb + t * a.bs[1], a.gate);
+        return x;
+    };
+    GdHop<T, R> next = fetch(0);
+    for (int t = 0; t < a.T; ++t) {
+        const GdHop<T, R> now = next;
+        if (t + 1 < a.T) next = fetch(t + 1);
+        const float alpha = __expf(now.g);
+        f32x4 sk = {0.f, 0.f, 0.f, 0.f}, sq = sk;
+        float qk = 0.f;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const float k = gd_load<T>(&now.k[j], 0), q = gd_load<T>(&now.q[j], 0);
+            qk = __builtin_fmaf(q, k, qk);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                S[j][i] *= alpha;
+                sk[i] = __builtin_fmaf(k, S[j][i], sk[i]);
+                sq[i] = __builtin_fmaf(q, S[j][i], sq[i]);
+            }
+        }
+#pragma unroll
+        for (int m = 8; m < 64; m <<= 1) {
+            qk += __shfl_xor(qk, m);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { sk[i] += __shfl_xor(sk[i], m); sq[i] += __shfl_xor(sq[i], m); }
+        }
+        f32x4 e, o;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { e[i] = now.beta * (gd_load<T>(&now.v[i], 0) - sk[i]); o[i] = a.scale * __builtin_fmaf(qk, e[i], sq[i]); }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const float k = gd_load<T>(&now.k[j], 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[j][i] = __builtin_fmaf(k, e[i], S[j][i]);
+        }
+        gd_put<T>(gd_buffer(a.out, ob + t * a.os[1], a.Dv, E), c0 * E, o, rg == 0 ? a.Dv - c0 : 0, WHOLE);
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) gd_put<float>(so, ((unsigned)(r0 + j) * a.Dv + c0) * 4, S[j], r0 + j < a.Dk ? a.Dv - c0 : 0, WHOLE);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------------------------
+// Clips: chunks of C frames.  With gamma = the running sum of g inside the chunk, d_ij = exp(gamma_i - gamma_j) and S the state before it,
+//     A_ij = beta_i d_ij k_i.k_j (j < i),   (I + A) u = beta (v - exp(gamma) (K S)),
+//     O = scale exp(gamma) (Q S) + P u,   P_ij = scale d_ij q_i.k_j (j <= i),   S <- exp(gamma_C) S + K^T (exp(gamma_C - gamma) u):
+// matrix products, and 16 dependent steps for the inverses of the 16 x 16 diagonal blocks of I + A where the definition has C.
+//
+// A workgroup is one head and 16 NW columns: wave w owns 16 columns of S, u and O in the matrix units' result layout (row 4 q + i, column n),
+// in which a result IS the next product's right operand -- K slot 8 q + 4 h + i of two 16-row blocks is row 4 q + i of block h -- so that
+// K S -> u -> P u, K^T u chain in registers, and the waves meet only over the chunk's K, Q, A and P in LDS, which are laid out in that order.
+//
+// Every fp32 operand goes in as bf16 limbs (split3 of gru_limb.h: exact), products of limbs whose indices add up to more than 2 (2^-24 of the
+// term) left out; bf16 values of k and q are one limb, fp16 two, fp32 three.  What only reaches the outputs of a 16-bit type (Q S, P u) takes two
+// limbs of either side, 2^-16 of a term against the 2^-8 and 2^-11 of the result's rounding; the state's path takes all.
+//
+// Where there are fewer heads than the chip holds workgroups, the frames are cut into segments.  A segment's effect on the state before it is
+// linear, S -> M S + N: MOVE runs a segment from S = 0 with its v (N) and from the unit matrix without (M, Dk columns more), no outputs;
+// gated_delta_join_kernel then walks the segments (N becomes the state that the next one starts with), and the segments run as
+// clips of their own.  About two and a half times the work, over `segments` times the workgroups.
+//
+// gamma and its differences are 64-bit: they are small differences of long sums.  A non-finite k, g or beta makes its head's outputs from its
+// frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all
+// frames of the chunk, so that such values are taken out of the operands first).
+// ---------------------------------------------------------------------------------------------------------------------------------------
+template <typename T> struct GdIn;
+template <> struct GdIn<__hip_bfloat16> { enum { L = 1 }; };
+template <> struct GdIn<__half> { enum { L = 2 }; };
+template <> struct GdIn<float> { enum { L = 3 }; };
+
+// the running sum over a wave's lanes
+__device__ __forceinline__ double gd_scan(double v) {
+#define GD_STEP_(ctrl, rows) { \
+        const unsigned long b = __builtin_bit_cast(unsigned long, v); \
+        const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)b, ctrl, rows, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(b >> 32), ctrl, rows, 0xf, false); \
+        v += __builtin_bit_cast(double, (unsigned long)hi << 32 | lo); }
+    GD_STEP_(0x111, 0xf) GD_STEP_(0x112, 0xf) GD_STEP_(0x114, 0xf) GD_STEP_(0x118, 0xf)      // row_shr 1, 2, 4, 8: inside 16 lanes
+    GD_STEP_(0x142, 0xa) GD_STEP_(0x143, 0xc)                                                // lane 15's sum to the next row, lane 31's to the upper half
+#undef GD_STEP_
+    return v;
 }
 // the row's limbs, 8 x 16 bit each; true where a value is not finite
 template <typename T> __device__ __forceinline__ bool gd_limbs(const GdRow<T>& r, uint4 (&f)[GdIn<T>::L]) {
@@ -297,7 +308,7 @@ __device__ __forceinline__ uint2 gd_column(const unsigned short* p) {
 
 // The clip that is `place`-th in a batch from long to short: thread i counts the clips before clip i, by chunks of 16 frames and number.  Workgroups
 // start in this order, so that no long clip begins when the others are done; the order has no part in the results.
-constexpr int GD_RANKED = 256;                             // clips of a batch that is put in order, the threads of the smaller workgroup
+constexpr int GD_RANKED = 256;                             // clips of a batch that is put in order, at most (and at most a workgroup's threads)
 __device__ __forceinline__ int gd_ranked(const GatedDeltaArgs& a, int place) {
     __shared__ __attribute__((aligned(16))) unsigned keys[GD_RANKED];
     __shared__ int found;
@@ -307,7 +318,7 @@ __device__ __forceinline__ int gd_ranked(const GatedDeltaArgs& a, int place) {
         const int n = a.lengths[i];
         mine = (n < 0 ? 0u : (unsigned)(n > a.T ? a.T : n) >> 4) << 8 | (255u - i);
     }
-    if (i < GD_RANKED) keys[i] = mine;
+    for (int j = i; j < GD_RANKED; j += blockDim.x) keys[j] = j == i ? mine : 0;
     __syncthreads();
     int before = 0;
 #pragma unroll 8
@@ -335,12 +346,12 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
     __shared__ __attribute__((aligned(16))) float eg[C], ee[C], bt[C];
     __shared__ int kbad[2];
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, q = lane >> 4;
-    const long unit = blockIdx.x / a.strips;               // (head, segment)
-    const int sg = (int)(unit % a.segments);
-    long head = unit / a.segments;
-    const long heads = (long)(gridDim.x / a.strips) / a.segments;
-    int b = (int)(head / a.Hv);
-    const int h = (int)(head - (long)b * a.Hv), hk = h / (a.Hv / a.Hk);
+    const unsigned unit = blockIdx.x / (unsigned)a.strips, place = unit / (unsigned)a.segments;               // (head, segment)
+    const int sg = (int)(unit - place * a.segments);
+    const long heads = gridDim.x / (unsigned)a.strips / (unsigned)a.segments;
+    int b = (int)(place / (unsigned)a.Hv);
+    const int h = (int)(place - (unsigned)b * a.Hv), hk = h / (a.Hv / a.Hk);
+    long head = place;
     if (!MOVE && a.sorted) { b = gd_ranked(a, b); head = (long)b * a.Hv + h; }
     int col = 16 * NW * (int)(blockIdx.x - unit * a.strips) + 16 * w + n;
     const int vcols = (a.Dv + 15) & ~15;
@@ -499,7 +510,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
             for (int l = 0; l < PL; ++l) Pf[(bi + 1) * (bi + 1) / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
         };
-        if (w < BLOCKS) blocks(w);
+        constexpr int FIRST = NW > CB ? NW < BLOCKS ? NW : BLOCKS : CB;
+        for (int e = w; e < FIRST; e += NW) blocks(e);
         __syncthreads();
         if (w == 0) {
             // lane (q, n): column n of block q, forward substitution, in place
@@ -516,7 +528,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 #pragma unroll
                 for (int i = 0; i < 16; ++i) D[i][n] = t[i];
         } else
-            for (int e = NW + w - 1; e < BLOCKS; e += NW - 1) blocks(e);
+            for (int e = FIRST + w - 1; e < BLOCKS; e += NW - 1) blocks(e);
         // x = K S, o = the transpose of Q S: frame n, columns 4 q ..
         f32x4 x[CB], o[MOVE ? 1 : CB];
         {
@@ -641,7 +653,7 @@ __global__ __launch_bounds__(4 * DKP) void gated_delta_join_kernel(GatedDeltaArg
     constexpr int NB = DKP / 16;
     __shared__ __attribute__((aligned(16))) float Sx[2][16][DKP + 4];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
-    const long head = blockIdx.x / a.strips;
+    const long head = blockIdx.x / (unsigned)a.strips;
     const int col = 16 * (int)(blockIdx.x - head * a.strips) + n, row = 16 * w + 4 * q;
     const bool cin = col < a.Dv;
     const long step = heads * a.Dk * a.Dv, sb = head * a.Dk * a.Dv + col;

@@ -82,22 +82,36 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
 }
 
 template <typename T>
-void gd_launch_step(const GatedDeltaArgs& a, unsigned grid, bool even, hipStream_t s) {
-#define GD_STEP(D) (even && a.Dk == D ? (gated_delta_step_kernel<T, D, true><<<grid, 64, 0, s>>>(a)) : (gated_delta_step_kernel<T, D, false><<<grid, 64, 0, s>>>(a)))
-    if (a.Dk <= 16) GD_STEP(16); else if (a.Dk <= 32) GD_STEP(32); else if (a.Dk <= 64) GD_STEP(64); else GD_STEP(128);
+void gd_launch_step(const GatedDeltaArgs& a, unsigned grid, hipStream_t s) {
+#define GD_STEP(D) (a.whole ? (gated_delta_step_kernel<T, D, true><<<grid, 64, 0, s>>>(a)) : (gated_delta_step_kernel<T, D, false><<<grid, 64, 0, s>>>(a)))
+    if (a.Dk <= 16) GD_STEP(16); else if (a.Dk <= 32) GD_STEP(32); else if (a.Dk <= 64) GD_STEP(64); else if (a.Dk <= 96) GD_STEP(96); else GD_STEP(128);
 #undef GD_STEP
 }
-// The frames of a chunk, the columns of a workgroup and the workgroups that a CU holds at once (registers and LDS)
+// Rows that can be read and written in pieces: whole fours of bytes
+bool gd_fours(const void* p, const long (&s)[3], int e) { return op_aligned(p, 4) && s[0] * e % 4 == 0 && s[1] * e % 4 == 0 && s[2] * e % 4 == 0; }
+void gd_pieces(GatedDeltaArgs& a, int e) {
+    a.whole = a.Dk % 8 == 0 && gd_fours(a.q, a.qs, e) && gd_fours(a.k, a.ks, e);
+    a.even = a.Dv % 4 == 0 && gd_fours(a.out, a.os, e);
+}
+// The frames of a chunk, the columns of a workgroup and the workgroups that a CU holds at once (registers and LDS).  Two waves for 32 columns
+// where a chunk has two diagonal blocks for them: with four, half of them would have no column (104 clips x 2463 frames, 8 heads of 16, fp32:
+// 683 us with four, 366 with two; fp16 with its four blocks, 166 clips x 450 frames: 107 with four, 120 with two).
 int gd_chunk(int dtype) { return dtype == DPDF_F32 ? 32 : 64; }
-int gd_columns(const GatedDeltaArgs& a) { return a.Dv <= 64 ? 64 : 128; }
-int gd_resident(const GatedDeltaArgs& a) { return a.Dv <= 64 && a.Dk <= 64 ? 2 : 1; }
-// Segments for `heads` heads: as many as fill the chip once, with four chunks at least each (their start state costs about one and a half times
-// their frames), and only where the chip would hold three times the workgroups there are.
-int gd_segments(const GatedDeltaArgs& a, long heads, int chunk, int cus) {
-    const long strips = (a.Dv + gd_columns(a) - 1) / gd_columns(a), groups = heads * strips, room = (long)cus * gd_resident(a);
-    const long chunks = ((long)a.T + chunk - 1) / chunk;
+int gd_columns(const GatedDeltaArgs& a, int dtype) { return a.Dv <= 32 && a.Dk <= 64 && dtype == DPDF_F32 ? 32 : a.Dv <= 64 ? 64 : 128; }
+int gd_resident(const GatedDeltaArgs& a, int dtype) {
+    const int columns = gd_columns(a, dtype);
+    return columns == 128 || (a.Dk > 64 && dtype == DPDF_F16) ? 1 : columns == 64 ? 2 : a.Dk <= 32 ? 4 : 3;
+}
+// Segments for `heads` heads: as many as fill the chip once, and only where the chip would hold three times the workgroups there are.  A segment costs
+// its frames about one and a half times more and a step of the join, a seventh of a chunk: hence no more than the root of five times the
+// chunks (6 heads, 48 chunks: 49 us in 12 segments, 45 in 16, 53 in 24), and at least two chunks each, four where the second pass would start in
+// several rounds (2 clips of 17 chunks, 4 heads: 36 us by two, 52 by four; 111 heads, 14 chunks: 150 and 106).
+int gd_segments(const GatedDeltaArgs& a, int dtype, long heads, int cus) {
+    const long strips = (a.Dv + gd_columns(a, dtype) - 1) / gd_columns(a, dtype), groups = heads * strips, room = (long)cus * gd_resident(a, dtype);
+    const long chunks = ((long)a.T + gd_chunk(dtype) - 1) / gd_chunk(dtype);
     long n = room / groups;
-    if (n > chunks / 4) n = chunks / 4;
+    if (n > chunks / (groups * 4 > cus ? 4 : 2)) n = chunks / (groups * 4 > cus ? 4 : 2);
+    while (n > 1 && n * n > 5 * chunks) --n;
     return n < 3 ? 1 : (int)n;
 }
 size_t gd_workspace(const GatedDeltaArgs& a, long heads, int segments) {
@@ -118,7 +132,11 @@ void gd_launch_clip(GatedDeltaArgs& a, long heads, hipStream_t s) {
 }
 template <typename T>
 void gd_launch_clips(GatedDeltaArgs& a, long heads, hipStream_t s) {
-#define GD_CLIP(D) (gd_columns(a) == 64 ? gd_launch_clip<T, D, 4>(a, heads, s) : gd_launch_clip<T, D, 8>(a, heads, s))
+    constexpr bool F32 = sizeof(T) == 4;
+    const int columns = gd_columns(a, F32 ? DPDF_F32 : DPDF_F16);
+#define GD_CLIP(D) (columns == 64 ? gd_launch_clip<T, D, 4>(a, heads, s) : gd_launch_clip<T, D, 8>(a, heads, s))
+    if constexpr (F32)
+        if (columns == 32) return a.Dk <= 32 ? gd_launch_clip<T, 32, 2>(a, heads, s) : gd_launch_clip<T, 64, 2>(a, heads, s);
     if (a.Dk <= 32) GD_CLIP(32); else if (a.Dk <= 64) GD_CLIP(64); else GD_CLIP(128);
 #undef GD_CLIP
 }
@@ -162,7 +180,7 @@ extern "C" size_t dpdf_gated_delta_workspace(int device, const dpdf_gated_delta_
     int cus = 0;
     if (gd_check(args, false, a) || !args->batch || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) return 0;
     const long heads = (long)args->batch * a.Hv;
-    return gd_workspace(a, heads, gd_segments(a, heads, gd_chunk(args->dtype), cus));
+    return gd_workspace(a, heads, gd_segments(a, args->dtype, heads, cus));
 }
 
 extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* workspace, size_t workspace_bytes, void* stream) {
@@ -174,11 +192,7 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
     for (const long* s : {args->q_stride, args->k_stride, args->v_stride, args->out_stride})
         if (s[1] > (most - (long)(a.Dk > a.Dv ? a.Dk : a.Dv) * e) / (rows * e)) return set_err(DPDF_E_INVALID, "gated delta rule: a stride of %ld from frame to frame is too large", s[1]);
     if (!op_aligned(workspace, 16)) return set_err(DPDF_E_INVALID, "gated delta rule: the workspace is not aligned to 16 bytes");
-    a.whole = a.Dk % 8 == 0;
-    for (const void* p : {a.q, a.k}) a.whole &= op_aligned(p, 4);
-    for (const long* s : {a.qs, a.ks}) for (int i = 0; i < 3; ++i) a.whole &= s[i] * e % 4 == 0;
-    a.even = a.Dv % 4 == 0 && op_aligned(a.out, 4);
-    for (int i = 0; i < 3; ++i) a.even &= a.os[i] * e % 4 == 0;
+    gd_pieces(a, (int)e);
     OpDevice dev(device);
     HIP_TRY(dev.err);
     const long heads = (long)args->batch * a.Hv, chunk = gd_chunk(args->dtype);
@@ -186,7 +200,7 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
     if (workspace) {
         int cus = 0;
         HIP_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
-        const int n = gd_segments(a, heads, (int)chunk, cus);
+        const int n = gd_segments(a, args->dtype, heads, cus);
         if (n > 1 && workspace_bytes >= gd_workspace(a, heads, n)) {
             const long chunks = (args->frames + chunk - 1) / chunk, each = (chunks + n - 1) / n;
             a.seg = (int)(each * chunk); a.segments = (int)((chunks + each - 1) / each);
@@ -199,11 +213,11 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
             a.starts = (float*)workspace; a.moves = a.starts + (size_t)a.segments * heads * a.Dk * a.Dv;
         }
     }
-    if (a.lengths && a.segments == 1 && a.B <= GD_RANKED && a.T < 1 << 25) {
+    if (a.lengths && a.segments == 1 && a.B <= 4 * gd_columns(a, args->dtype) && a.B <= GD_RANKED && a.T < 1 << 25) {
         int cus = 0;
         HIP_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
         // all of them start at once otherwise (256 clips of 334 to 1003 frames, 4 heads of 64 in bf16: 205 us in the batch's order, 178 us so)
-        a.sorted = heads * ((a.Dv + gd_columns(a) - 1) / gd_columns(a)) > (long)cus * gd_resident(a);
+        a.sorted = heads * ((a.Dv + gd_columns(a, args->dtype) - 1) / gd_columns(a, args->dtype)) > (long)cus * gd_resident(a, args->dtype);
     }
     gd_type(args->dtype, [&](auto t) { gd_launch_clips<decltype(t)>(a, heads, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());
@@ -214,12 +228,15 @@ extern "C" int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* ar
     GatedDeltaArgs a;
     if (int rc = gd_check(args, true, a)) return rc;
     if (!args->batch || !args->frames) return DPDF_OK;
+    // a head's state is addressed with 32 bits
+    if ((long)a.Dk * a.Dv > (1L << 28)) return set_err(DPDF_E_INVALID, "gated delta rule: a head of %d x %d is too large", a.Dk, a.Dv);
+    gd_pieces(a, op_bytes(args->dtype));
+    a.whole &= a.even && gd_fours(a.v, a.vs, op_bytes(args->dtype));
     OpDevice dev(device);
     HIP_TRY(dev.err);
     a.strips = (a.Dv + 31) / 32;
     const unsigned grid = (unsigned)((long)args->batch * a.Hv * a.strips);
-    const bool even = a.Dv % 32 == 0 && op_aligned(a.state_in, 16) && op_aligned(a.state_out, 16);
-    gd_type(args->dtype, [&](auto t) { gd_launch_step<decltype(t)>(a, grid, even, (hipStream_t)stream); });
+    gd_type(args->dtype, [&](auto t) { gd_launch_step<decltype(t)>(a, grid, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());
     return DPDF_OK;
 }

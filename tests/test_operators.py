@@ -147,6 +147,11 @@ def test_gated_delta_refusals(change, word):
 
 
 def test_gated_delta_step_refusals_and_empty_calls():
+    one = dict(batch=1, frames=1, k_heads=1, v_heads=1, k_dim=128, state_in=1 << 50, state_out=1 << 50, v=1 << 51, out=1 << 52)
+    for n in ("q", "k", "v", "g", "beta", "out"):
+        one[n + "_stride"] = (1 << 22,) * 3
+    rc, msg = _c_gated(step=True, v_dim=1 << 22, **one)
+    assert rc == -1 and "128 x 4194304 is too large" in msg, (rc, msg)
     assert _c_gated(step=True, lengths=0x8000000)[0] == -1
     assert _c_gated(step=True, state_in=None)[0] == -1 and _c_gated(step=True, state_out=None)[0] == -1
     L = backend.load_library()
@@ -256,6 +261,23 @@ def test_steps_against_the_definition(shape, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("S, T, Hk, Hv, Dk, Dv", [(3, 4, 1, 2, 96, 40), (2, 3, 2, 2, 80, 100), (5, 2, 1, 1, 72, 3), (2, 5, 1, 3, 67, 33), (1, 6, 2, 4, 88, 16), (2, 2, 1, 1, 20, 36), (3, 3, 1, 1, 8, 1)])
+def test_steps_of_sizes_between(S, T, Hk, Hv, Dk, Dv, dtype):
+    x = inputs(S, T, Hk, Hv, Dk, Dv, dtype, seed=Dk + Dv)
+    room = torch.full((S * Hv * Dk * Dv + 64,), math.nan, device="cuda")                # nothing beside the state is taken for it or written
+    state = room[32:-32].view(S, Hv, Dk, Dv)
+    state.copy_(0.5 * torch.randn(S, Hv, Dk, Dv, generator=torch.Generator().manual_seed(1)))
+    ref, rend = delta_rule(*x, state=state)
+    wide = torch.full((S, T, Hv, Dv + 5), 3.0, dtype=dtype, device="cuda")
+    out = operators.gated_delta_step(*x, state, out=wide[..., 2:Dv + 2])
+    near(out, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
+    near(state, rend, tol(T, Dk))
+    assert bool(room[:32].isnan().all()) and bool(room[-32:].isnan().all())
+    assert bool((wide[..., :2] == 3).all()) and bool((wide[..., Dv + 2:] == 3).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_gates_of_the_values_type(dtype):
     x = inputs(2, 100, 2, 2, 32, 32, dtype, seed=4)
@@ -323,14 +345,14 @@ def test_ragged_clips_leave_the_rest_alone(lens):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("B, T, lens", [(256, 40, "any"), (200, 70, "any"), (180, 33, "equal"), (257, 20, "any")])
-def test_many_clips_of_any_lengths(B, T, lens, dtype):
+@pytest.mark.parametrize("B, T, lens, D", [(256, 40, "any", 48), (200, 70, "any", 64), (180, 33, "equal", 48), (257, 20, "any", 48), (128, 66, "any", 32), (129, 35, "any", 20), (100, 65, "any", 130)])
+def test_many_clips_of_any_lengths(B, T, lens, D, dtype):
     """More clips than start at once, whatever order they are started in."""
-    x = inputs(B, T, 2, 4, 16, 32, dtype, seed=B)
+    x = inputs(B, T, 2, 8, 16, D, dtype, seed=B)
     gen = torch.Generator().manual_seed(B)
     n = torch.full((B,), 17) if lens == "equal" else torch.randint(-3, T + 4, (B,), generator=gen)
     n = n.to(torch.int32)
-    out = torch.full((B, T, 4, 32), 5.0, dtype=dtype, device="cuda")
+    out = torch.full((B, T, 8, D), 5.0, dtype=dtype, device="cuda")
     got, end = operators.gated_delta(*x, lengths=n.cuda(), out=out)
     ref, rend = delta_rule(*x, lengths=n.clamp(0, T))
     on = (torch.arange(T)[None] < n[:, None]).cuda()
