@@ -262,6 +262,18 @@ def test_steps_against_the_definition(shape, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("Dk", [8, 16, 13, 24, 31, 40, 63, 72, 96, 95, 104, 128, 127])
+def test_steps_of_every_size(Dk, dtype):
+    x = inputs(2, 3, 1, 2, Dk, 36, dtype, seed=Dk)
+    state = 0.5 * torch.randn(2, 2, Dk, 36, generator=torch.Generator().manual_seed(1)).cuda()
+    ref, rend = delta_rule(*x, state=state)
+    out = operators.gated_delta_step(*x, state)
+    near(out, ref, tol(3, Dk), HALF_STEP[dtype], TINY[dtype])
+    near(state, rend, tol(3, Dk))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("S, T, Hk, Hv, Dk, Dv", [(3, 4, 1, 2, 96, 40), (2, 3, 2, 2, 80, 100), (5, 2, 1, 1, 72, 3), (2, 5, 1, 3, 67, 33), (1, 6, 2, 4, 88, 16), (2, 2, 1, 1, 20, 36), (3, 3, 1, 1, 8, 1)])
 def test_steps_of_sizes_between(S, T, Hk, Hv, Dk, Dv, dtype):
     x = inputs(S, T, Hk, Hv, Dk, Dv, dtype, seed=Dk + Dv)
@@ -518,6 +530,20 @@ def test_few_long_clips_are_cut_into_segments(T, lens, Hk, Hv, Dk, Dv, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("Dv", [20, 60, 100])
+@pytest.mark.parametrize("Dk", [20, 50, 100])
+def test_long_clips_of_every_size(Dk, Dv, dtype):
+    T = 600
+    x = inputs(1, T, 1, 2, Dk, Dv, dtype, seed=Dk + Dv)
+    state = 0.5 * torch.randn(1, 2, Dk, Dv, generator=torch.Generator().manual_seed(2)).cuda()
+    out, end = operators.gated_delta(*x, state=state)
+    ref, rend = delta_rule(*x, state=state)
+    near(out, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
+    near(end, rend, tol(T, Dk))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["k", "v", "beta"])
 @pytest.mark.parametrize("at", [0, 700, 1199])
 def test_a_non_finite_value_in_a_clip_of_segments(what, at):
@@ -641,6 +667,19 @@ def test_w4_layers_against_the_definition(M, K, N, group, dtype):
         for b in (None, bias):
             ref, mag = w4_layer(x, codes, scales, z, b, group)
             near_layer(operators.w4_matvec(x, codes, scales, zeros=z, bias=b, group=group), ref, mag, K, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, scale_dtype", [(F32, F32), (F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("M, N", [(3, 1000), (2, 16400), (17, 8200), (5, 32800), (40, 11000)])
+@pytest.mark.parametrize("K, group", [(130, 32), (700, 64), (1300, 128), (1100, 96)])
+def test_w4_layers_of_many_outputs(M, N, K, group, dtype, scale_dtype):
+    """Every number of tiles to a workgroup, of waves and of blocks to a wave; rows of x in more than one tile."""
+    x, codes, scales, z, bias = layer(M, K, N, group, dtype, K == 700, seed=N, scale_dtype=scale_dtype)
+    y = operators.w4_matvec(x, codes, scales, zeros=z, bias=bias, group=group)
+    at = torch.cat([torch.arange(0, N, 97), torch.arange(N - 40, N)]).cuda()             # outputs are independent: some of all tiles, and the last
+    ref, mag = w4_layer(x, codes[at], scales[at], None if z is None else z[at], bias[at], group)
+    near_layer(y[:, at], ref, mag, K, dtype)
 
 
 @pytest.mark.gpu
