@@ -23,6 +23,7 @@ from __future__ import annotations
 import argparse
 import json
 import os
+import signal
 import subprocess
 import sys
 import threading
@@ -727,12 +728,16 @@ def dist_selftest(timeout_s: float = 60.0) -> dict:
     return res
 
 
-def reexec_with_gloo_fallback(reason: str) -> None:
-    """RCCL did not come up (or stopped answering) on this node: replace THIS rank's process image with the same command line on
-    `--backend gloo --fallback-reason ...` (same PID, so the launcher that watches the rank sees nothing die).  Every rank gets
-    here on its own -- by its watchdog, or by the exception RCCL raised -- and they meet again at a fresh TCP rendezvous one
-    port above the launcher's.  The line then says `collective: "FALLBACK gloo: <reason>"`, the per-GPU compute figures are
+_FALLBACK = threading.Lock()             # taken by the thread that falls back, for good: every other one waits for the process's end
+
+
+def rerun_with_gloo_fallback(reason: str) -> None:
+    """RCCL did not come up (or stopped answering) on this node: run the same command line on `--backend gloo --fallback-reason ...` as a child
+    process and end with its exit code (a process that has initialised the GPU is not replaced by another program; the launcher that
+    watches this rank sees nothing die).  Every rank gets here on its own -- by its watchdog, or by the exception RCCL raised -- and they
+    meet again at a fresh TCP rendezvous one port above the launcher's.  The line then says `collective: "FALLBACK gloo: <reason>"`, the per-GPU compute figures are
     still measured, rc stays 0."""
+    _FALLBACK.acquire()
     argv = [a for a in sys.argv[1:]]
     out, skip = [], False
     for a in argv:
@@ -748,15 +753,19 @@ def reexec_with_gloo_fallback(reason: str) -> None:
     reason = " ".join(str(reason).split())[:300]
     env = dict(os.environ)
     env.setdefault("DPDF_BENCH_FALLBACK_PORT", str(int(env.get("MASTER_PORT", "29500")) + 17))
-    print(f"[bench.py] rank {env.get('RANK', '0')}: RCCL unusable ({reason}); re-executing on --backend gloo (control plane + host-staged "
+    print(f"[bench.py] rank {env.get('RANK', '0')}: RCCL unusable ({reason}); running again on --backend gloo (control plane + host-staged "
           f"gather), rendezvous 127.0.0.1:{env['DPDF_BENCH_FALLBACK_PORT']}", file=sys.stderr, flush=True)
     sys.stdout.flush()
-    os.execve(sys.executable, [sys.executable, str(Path(__file__).resolve())] + out + ["--backend", "gloo", "--fallback-reason", reason], env)
+    rc = 1
+    try:
+        rc = subprocess.call([sys.executable, str(Path(__file__).resolve())] + out + ["--backend", "gloo", "--fallback-reason", reason], env=env)
+    finally:
+        os._exit(rc if 0 <= rc < 256 else 1)      # the main thread may be stuck inside RCCL
 
 
 class CollectiveWatchdog:
-    """A hang inside RCCL (communicator init, a collective whose peer never arrives) raises nothing: a timer thread re-executes the
-    rank on the gloo fallback when the watched section overruns its deadline.  `stage()` names what is running (it goes on the
+    """A hang inside RCCL (communicator init, a collective whose peer never arrives) raises nothing: a timer thread runs the
+    rank again on the gloo fallback when the watched section overruns its deadline.  `stage()` names what is running (it goes on the
     line as the reason); `disarm()` ends the watch."""
 
     def __init__(self) -> None:
@@ -781,9 +790,11 @@ class CollectiveWatchdog:
             if self._timer is not None:
                 self._timer.cancel()
                 self._timer = None
+        with _FALLBACK:                  # an answer that comes once the fallback runs is too late
+            pass
 
     def _fire(self, seconds: float) -> None:
-        reexec_with_gloo_fallback(f"no answer within {seconds:g} s at stage `{self._stage}`")
+        rerun_with_gloo_fallback(f"no answer within {seconds:g} s at stage `{self._stage}`")
 
 
 def float64_recurrence_error() -> dict:
@@ -855,8 +866,11 @@ def main() -> None:
     ap.add_argument("--ref-slots", default="", help=argparse.SUPPRESS)
     ap.add_argument("--public-streams-only", default="", help=argparse.SUPPRESS)
     ap.add_argument("--side-config", default="", help=argparse.SUPPRESS)
-    ap.add_argument("--fallback-reason", default="", help=argparse.SUPPRESS)      # set by reexec_with_gloo_fallback
+    ap.add_argument("--fallback-reason", default="", help=argparse.SUPPRESS)      # set by rerun_with_gloo_fallback
     args = ap.parse_args()
+    if args.fallback_reason and sys.platform == "linux":
+        import ctypes
+        ctypes.CDLL(None).prctl(1, int(signal.SIGTERM), 0, 0, 0)        # PR_SET_PDEATHSIG: the launcher ends the rank that started this process
 
     if args.side_config == "all":
         print("SIDE " + json.dumps(side_all()), flush=True)
@@ -921,7 +935,7 @@ def main() -> None:
         os.environ.setdefault("MASTER_ADDR", "127.0.0.1")
         if args.backend == "nccl":
             # communicator init + the first collectives under a watchdog: RCCL hangs raise nothing (round 4: a ONE-rank init sat
-            # for 180 s on the driver's box); overrun or exception -> the rank re-executes itself on the gloo fallback
+            # for 180 s on the driver's box); overrun or exception -> the rank runs again on the gloo fallback
             try:
                 wd.arm(wd_s, "init_process_group(nccl, device_id)")
                 if fake_hang:
@@ -943,7 +957,7 @@ def main() -> None:
                 raise
             except Exception as exc:
                 wd.disarm()
-                reexec_with_gloo_fallback(f"{type(exc).__name__} at stage `{wd._stage}`: {exc}")
+                rerun_with_gloo_fallback(f"{type(exc).__name__} at stage `{wd._stage}`: {exc}")
         elif args.fallback_reason:
             # an explicit store: under torch.distributed.run (TORCHELASTIC_USE_AGENT_STORE) a tcp:// init_method makes EVERY rank a
             # client of a store nobody hosts -- both ranks sat in the rendezvous for good (found by the fake-hang GPU test)
@@ -998,7 +1012,7 @@ def main() -> None:
     out = torch.empty_like(wav)
     gathered = None
     do_gather = world > 1 and not args.no_gather
-    fallback = bool(args.fallback_reason)                 # this rank was re-executed on gloo because RCCL did not answer
+    fallback = bool(args.fallback_reason)                 # this rank runs again on gloo because RCCL did not answer
     gather_note = "none (single GPU)" if world == 1 else ((("rccl" if args.backend == "nccl" else args.backend) + " gather to rank 0") if do_gather else "disabled")
     if fallback:
         gather_note = (f"FALLBACK gloo: {args.fallback_reason}; barriers / clocks over gloo, the enhanced PCM gathered to rank 0 over gloo through "
