@@ -29,6 +29,9 @@ struct W4Args {
 // 32 in a row: one group whatever its size, and x is read 64 bytes of a row at a time.  R such products are of one group: 4 where 128
 // divides the group, 2 where 64 does, else 1.  Scales and zeros are read for four blocks at once, those of block q by lane (q, n), and go through
 // LDS as fp32: read block by block, 2 bytes of 16 rows at a time, they cost more than the codes (8192 x 32768: 25 of 72 us).
+//
+// Bound: reading the codes; what keeps it from a plain read's rate (24.6 us for the codes of 8192 x 32768, 5.5 TB/s) is the traffic beside them,
+// x about 7 us and scales 5.  8192 x 32768, eight rows of bf16: 44 us, 3.2 TB/s; 4096 x 16384, one row: 11.7 us, 3.0 TB/s; 4096 x 4096, 16 rows: 8.1 us.
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 template <typename T> struct W4X;                 // eight inputs of a row as a left operand: LIMBS fragments

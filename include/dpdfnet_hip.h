@@ -214,8 +214,9 @@ enum { DPDF_F32 = 0, DPDF_F16 = 1, DPDF_BF16 = 2 };
 /* The gated delta rule, a recurrence over frames with a matrix state S [k_dim][v_dim] per sequence and value head:
  *   S' = exp(g_t) S_{t-1};  e_t = beta_t (v_t - S'^T k_t);  S_t = S' + k_t e_t^T;  out_t = scale S_t^T q_t
  * q, k [batch, frames, k_heads, k_dim]; v, out [batch, frames, v_heads, v_dim]; g, beta [batch, frames, v_heads];
- * state_in, state_out [batch, v_heads, k_dim, v_dim] fp32, contiguous.  Clips: 64 frames of a tensor span less than 2 GiB.  k_dim 1 .. 128; v_heads a multiple of k_heads, value head h reads
- * key head h / (v_heads / k_heads).  The state is held, and every sum taken, in fp32.  g = -inf resets the state. */
+ * state_in, state_out [batch, v_heads, k_dim, v_dim] fp32, contiguous.  Clips: 64 frames of a tensor span less than 2 GiB.  k_dim 1 .. 128;
+ * v_heads a multiple of k_heads, value head h reads key head h / (v_heads / k_heads).  The state is held, and every sum taken, in fp32.
+ * g = -inf resets the state. */
 typedef struct dpdf_gated_delta_args {
     int dtype, gate_dtype;                   /* of q, k, v, out; of g, beta: DPDF_F32 or dtype */
     int batch, frames, k_heads, v_heads, k_dim, v_dim;
@@ -231,19 +232,21 @@ typedef struct dpdf_gated_delta_args {
 
 /* Whole clips, in chunks of 32 or 64 frames.  Frames behind a clip's length are neither read nor written; state_out is the state after its last
  * frame (a clip of length 0: the state it came with).  A non-finite k, g (but -inf) or beta makes the outputs of its head from its frame
- * on, and its state, NaN, a non-finite v those of its column, a non-finite q those of its frame; nothing earlier and no other head. */
-/* Few heads over many frames are cut into segments that run side by side, given a workspace for the segments' states:
+ * on, and its state, NaN, a non-finite v those of its column, a non-finite q those of its frame; nothing earlier and no other head.
+ *
+ * Few heads over many frames are cut into segments that run side by side, given a workspace for the segments' states:
  * dpdf_gated_delta_workspace() bytes on the device, aligned to 16, the call's alone until it has run; 0 where there is nothing to cut.
  * With less (or NULL) the clips run in one piece: the same results to rounding, slower. */
 size_t dpdf_gated_delta_workspace(int device, const dpdf_gated_delta_args* args);
 int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* `frames` hops (one, or a few) of every active stream, frame by frame; state_in is required, state_out = state_in updates it in place.
- * Rows of streams that are left out are neither read nor written. */
+ * Rows of streams that are left out are neither read nor written.  k_dim x v_dim at most 2^28. */
 int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* args, void* stream);
 
 /* Dense layers with 4-bit weights: out[m][n] = sum_k x[m][k] (code[n][k] - zero[n][k / group]) scale[n][k / group] + bias[n], sums in fp32.
  * Codes are two to a byte, the lower half first (codes [out_dim, (in_dim + 1) / 2]); scales, zeros [out_dim, ceil(in_dim / group)];
- * group a multiple of 32, the last one may be short. */
+ * group a multiple of 32, the last one may be short.  A value of x that is not finite makes its row's outputs so (NaN where the formula has an
+ * infinity), a scale its output's. */
 typedef struct dpdf_w4_matvec_args {
     int dtype, scale_dtype;                  /* of x, bias, out; of scales: DPDF_F32 or dtype */
     int rows, in_dim, out_dim, group;
