@@ -76,6 +76,8 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
         a.qs[i] = x.q_stride[i]; a.ks[i] = x.k_stride[i]; a.vs[i] = x.v_stride[i];
         a.gs[i] = x.g_stride[i]; a.bs[i] = x.beta_stride[i]; a.os[i] = x.out_stride[i];
     }
+    // one frame has no next one: its step may be anything, but the rows that a chunk has behind it must lie behind it
+    if (x.frames == 1) { a.qs[1] = a.ks[1] = Dk; a.vs[1] = a.os[1] = Dv; }
     a.B = x.batch; a.T = x.frames; a.Hk = x.k_heads; a.Hv = x.v_heads; a.Dk = x.k_dim; a.Dv = x.v_dim; a.scale = x.scale; a.gate = x.gate_dtype;
     a.segments = 1; a.seg = 0; a.starts = a.moves = nullptr; a.whole = a.even = a.sorted = 0; a.strips = 0;
     return DPDF_OK;
@@ -187,10 +189,10 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
     GatedDeltaArgs a;
     if (int rc = gd_check(args, false, a)) return rc;
     if (!args->batch || (!args->frames && !args->state_out)) return DPDF_OK;
-    // a chunk's rows are addressed with 32 bits
-    const long most = (1L << 31) - 1, rows = args->frames < 1 ? 1 : args->frames < 64 ? args->frames : 64, e = op_bytes(args->dtype);
-    for (const long* s : {args->q_stride, args->k_stride, args->v_stride, args->out_stride})
-        if (s[1] > (most - (long)(a.Dk > a.Dv ? a.Dk : a.Dv) * e) / (rows * e)) return set_err(DPDF_E_INVALID, "gated delta rule: a stride of %ld from frame to frame is too large", s[1]);
+    // a chunk's rows, also those behind the last frame, are addressed with 32 bits
+    const long most = (1L << 31) - 1, e = op_bytes(args->dtype);
+    for (const long* s : {a.qs, a.ks, a.vs, a.os})
+        if (s[1] > (most - (long)(a.Dk > a.Dv ? a.Dk : a.Dv) * e) / (64 * e)) return set_err(DPDF_E_INVALID, "gated delta rule: a stride of %ld from frame to frame is too large", s[1]);
     if (!op_aligned(workspace, 16)) return set_err(DPDF_E_INVALID, "gated delta rule: the workspace is not aligned to 16 bytes");
     gd_pieces(a, (int)e);
     OpDevice dev(device);

@@ -140,6 +140,7 @@ def _c_gated(step=False, workspace=None, **change):
     (dict(state_out=0x7000004), "in part"), (dict(state_out=0x2000000), "overlaps an input"), (dict(active=0x9000000), "mask"),
     (dict(batch=1 << 30), "too large"), (dict(frames=(1 << 30) + 1), "too large"), (dict(workspace=0x9000008), "aligned"),
  (dict(k=1 << 45, k_stride=(1 << 38, 1 << 30, 16)), "frame to frame"), (dict(out=1 << 45, out_stride=(1 << 40, 1 << 31, 8)), "frame to frame"),
+    (dict(frames=2, out=1 << 45, out_stride=(1 << 40, 1 << 25, 8)), "frame to frame"), (dict(frames=2, v=1 << 45, v_stride=(1 << 40, 1 << 24, 8)), "frame to frame"),
 ])
 def test_gated_delta_refusals(change, word):
     rc, msg = _c_gated(**change)
@@ -374,6 +375,24 @@ def test_many_clips_of_any_lengths(B, T, lens, D, dtype):
     alone = [operators.gated_delta(*(t[b:b + 1] for t in x), lengths=n[b:b + 1].cuda()) for b in (0, 1, B - 1)]
     for (o, e), b in zip(alone, (0, 1, B - 1)):
         assert torch.equal(e[0], end[b]) and torch.equal(o[0][on[b]], got[b][on[b]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("step", [0, 1, 5])
+def test_one_frame_whose_step_says_nothing(step, dtype):
+    """Tensors of one frame may have any stride from frame to frame."""
+    x = inputs(2, 1, 1, 2, 24, 20, dtype, seed=step)
+    ref, rend = delta_rule(*x)
+    q, k, v = (t.as_strided(t.shape, (t.stride(0), step, *t.stride()[2:])) for t in x[:3])
+    out = torch.full((2, 1, 2, 20), 7.0, dtype=dtype, device="cuda")
+    got, end = operators.gated_delta(q, k, v, *x[3:], out=out.as_strided(out.shape, (40, step, 20, 1)))
+    near(got, ref, tol(1, 24), HALF_STEP[dtype], TINY[dtype])
+    near(end, rend, tol(1, 24))
+    state = torch.zeros_like(end)
+    got = operators.gated_delta_step(q, k, v, *x[3:], state, out=out.as_strided(out.shape, (40, step, 20, 1)))
+    near(got, ref, tol(1, 24), HALF_STEP[dtype], TINY[dtype])
+    near(state, rend, tol(1, 24))
 
 
 @pytest.mark.gpu
