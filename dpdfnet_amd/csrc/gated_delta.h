@@ -211,8 +211,8 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
 // K S -> u -> P u, K^T u chain in registers, and the waves meet only over the chunk's K, Q, A and P in LDS, which are laid out in that order.
 //
 // Every fp32 operand goes in as bf16 limbs (split3 of gru_limb.h: exact), products of limbs whose indices add up to more than 2 (2^-24 of the
-// term) left out; bf16 values of k and q are one limb, fp16 two, fp32 three.  What only reaches the outputs of a 16-bit type (Q S, P u) takes two
-// limbs of either side, 2^-16 of a term against the 2^-8 and 2^-11 of the result's rounding; the state's path takes all.
+// term) left out; bf16 values of k and q are one limb, fp16 two, fp32 three.  Outputs of 16 bits take as many limbs as the state's path: where a key
+// is written again, Q S and P u cancel, and what counts is 2^-24 of the terms, not the rounding of the result.
 //
 // Where there are fewer heads than the chip holds workgroups, the frames are cut into segments.  A segment's effect on the state before it is
 // linear, S -> M S + N: MOVE runs a segment from S = 0 with its v (N) and from the unit matrix without (M, Dk columns more), no outputs;
@@ -221,8 +221,9 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
 //
 // Bound: neither bytes nor products but the chain through a chunk, about 14 thousand cycles of which two workgroups on a CU overlap: K and Q into LDS
 // 1.4 thousand, the next chunk's loads 1 to 1.8, the blocks of A and P 1.8, inverses and the other blocks 2, K S and Q S 2, u, the outputs
-// and S 5 (4 heads of 64, bf16; vector units 42 % busy, matrix units 27 %).  256 clips of 334 to 1003 frames, 4 heads of 64, bf16: 174 us, 2.1 TB/s;
-// one recording of 16384 frames, 16 heads of 128: 396 us, in 16 segments (2.2 ms in one).  Chunks of 32 frames in 16-bit types: 228 and 532 us.
+// and S 5 (4 heads of 64, bf16; vector units 42 % busy, matrix units 27 %; outputs then had two limbs, 174 us).  256 clips of 334 to 1003
+// frames, 4 heads of 64, bf16: 193 us, 1.9 TB/s; one recording of 16384 frames, 16 heads of 128: 413 us, in 16 segments.  With outputs of two
+// limbs these took 174 and 396 us (2.2 ms in one segment), and chunks of 32 frames in 16-bit types 228 and 532.
 //
 // gamma and its differences are 64-bit: they are small differences of long sums.  A non-finite k, g or beta makes its head's outputs from its
 // frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all
@@ -273,10 +274,10 @@ template <int N> __device__ __forceinline__ void gd_split(const f32x4& v, uint4 
         if (l + 1 < N) { r0 -= bf_lo(p); r1 -= bf_hi(p); r2 -= bf_lo(s); r3 -= bf_hi(s); }
     }
 }
-// acc + a b over 32 slots, NA limbs by NB limbs, pairs up to TOP
-template <int TOP, int NA, int NB> __device__ __forceinline__ f32x4 gd_mul(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 acc) {
+// acc + a b over 32 slots, NA limbs by NB limbs, pairs up to 2
+template <int NA, int NB> __device__ __forceinline__ f32x4 gd_mul(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 acc) {
 #pragma unroll
-    for (int o = TOP; o >= 0; --o)
+    for (int o = 2; o >= 0; --o)
 #pragma unroll
         for (int l = 0; l < NA; ++l)
             if (o - l >= 0 && o - l < NB) acc = mfma_bf16(a[l], b[o - l], acc);
@@ -291,17 +292,17 @@ __device__ __forceinline__ f32x4 gd_mul16(const uint2 (&a)[3], const uint4* b, f
     return mfma_bf16(a01, gd_two(b[0], b[0]), acc);
 }
 // The transposes of such products: the two operands' layouts are the same, so the other order gives the transpose, a lane four columns of a row.
-template <int TOP, int NA, int NB> __device__ __forceinline__ f32x4 gd_mul_t(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 acc) {
+template <int NA, int NB> __device__ __forceinline__ f32x4 gd_mul_t(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 acc) {
 #pragma unroll
-    for (int o = TOP; o >= 0; --o)
+    for (int o = 2; o >= 0; --o)
 #pragma unroll
         for (int l = 0; l < NA; ++l)
             if (o - l >= 0 && o - l < NB) acc = mfma_bf16(b[o - l], a[l], acc);
     return acc;
 }
-template <int N> __device__ __forceinline__ f32x4 gd_mul16_t(const uint2 (&a)[N], const uint4* b, f32x4 acc) {
+__device__ __forceinline__ f32x4 gd_mul16_t(const uint2 (&a)[3], const uint4* b, f32x4 acc) {
     const uint4 a01 = make_uint4(a[0].x, a[0].y, a[1].x, a[1].y);
-    if constexpr (N == 3) acc = mfma_bf16(gd_two(b[2], b[0]), make_uint4(a[0].x, a[0].y, a[2].x, a[2].y), acc);
+    acc = mfma_bf16(gd_two(b[2], b[0]), make_uint4(a[0].x, a[0].y, a[2].x, a[2].y), acc);
     acc = mfma_bf16(gd_two(b[1], b[1]), a01, acc);
     return mfma_bf16(gd_two(b[0], b[0]), a01, acc);
 }
@@ -340,12 +341,11 @@ template <typename T, int DKP, int NW, int C, bool MOVE>
 __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDeltaArgs a) {
     constexpr int L = GdIn<T>::L, NB = DKP / 16, NC = DKP / 32, CB = C / 16, CC = C / 32, LDK = DKP + 8, E = sizeof(T);
     constexpr int BLOCKS = CB * (CB + 1) / 2;
-    constexpr bool WIDE = E == 4;                          // outputs of 32 bits
-    constexpr int PL = WIDE ? 3 : 2, ITEMS = (C / 2 * (DKP / 8) + 64 * NW - 1) / (64 * NW);
+    constexpr int ITEMS = (C / 2 * (DKP / 8) + 64 * NW - 1) / (64 * NW);
     // blocks of A below the diagonal and of P on and below it, two neighbours of a row to a fragment: row bi of A starts at bi^2 / 4, of P at (bi + 1)^2 / 4
     constexpr int ASLOTS = CB * CB / 4, PSLOTS = (CB + 1) * (CB + 1) / 4;
     __shared__ __attribute__((aligned(16))) unsigned short Kr[L][C][LDK], Qr[MOVE ? 1 : L][MOVE ? 1 : C][LDK];
-    __shared__ __attribute__((aligned(16))) uint2 Af[ASLOTS][3][64][2], Pf[MOVE ? 1 : PSLOTS][PL][64][2];
+    __shared__ __attribute__((aligned(16))) uint2 Af[ASLOTS][3][64][2], Pf[MOVE ? 1 : PSLOTS][3][64][2];
     __shared__ __attribute__((aligned(16))) float Ad[CB][16][20];
     __shared__ __attribute__((aligned(16))) float2 gam[C];
     __shared__ __attribute__((aligned(16))) float eg[C], ee[C], bt[C];
@@ -483,8 +483,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                     ki[l] = *(const uint4*)&Kr[l][16 * bi + n][32 * c + 8 * q];
                     if constexpr (!MOVE) qi[l] = *(const uint4*)&Qr[l][16 * bi + n][32 * c + 8 * q];
                 }
-                xa = gd_mul<2>(kj, ki, xa);
-                if constexpr (!MOVE) xp = gd_mul<2>(kj, qi, xp);
+                xa = gd_mul(kj, ki, xa);
+                if constexpr (!MOVE) xp = gd_mul(kj, qi, xp);
             }
             const float2 gr = gam[16 * bi + n];
             const float br = -bt[16 * bi + n];
@@ -510,10 +510,10 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 for (int l = 0; l < 3; ++l) Af[bi * bi / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
             }
             if constexpr (MOVE) return;
-            uint4 f[PL];
+            uint4 f[3];
             gd_split(xp, f, 0);
 #pragma unroll
-            for (int l = 0; l < PL; ++l) Pf[(bi + 1) * (bi + 1) / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
+            for (int l = 0; l < 3; ++l) Pf[(bi + 1) * (bi + 1) / 4 + bj / 2][l][lane][bj & 1] = make_uint2(f[l].x, f[l].y);
         };
         constexpr int FIRST = NW > CB ? NW < BLOCKS ? NW : BLOCKS : CB;
         for (int e = w; e < FIRST; e += NW) blocks(e);
@@ -552,8 +552,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                         kf[l] = *(const uint4*)&Kr[l][16 * bl + n][32 * c + 8 * q];
                         if constexpr (!MOVE) qf[l] = *(const uint4*)&Qr[l][16 * bl + n][32 * c + 8 * q];
                     }
-                    x[bl] = gd_mul<2>(kf, sl[c], x[bl]);
-                    if constexpr (!MOVE) o[bl] = gd_mul_t<WIDE ? 2 : 1>(qf, sl[c], o[bl]);
+                    x[bl] = gd_mul(kf, sl[c], x[bl]);
+                    if constexpr (!MOVE) o[bl] = gd_mul_t(qf, sl[c], o[bl]);
                 }
             }
         }
@@ -585,7 +585,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 uint4 f[3];
 #pragma unroll
                 for (int l = 0; l < 3; ++l) f[l] = *(const uint4*)Af[bl * bl / 4 + c][l][lane];
-                z = gd_mul<2>(f, ul[c], z);
+                z = gd_mul(f, ul[c], z);
             }
             if (bl & 1) {
                 uint2 f[3];
@@ -601,15 +601,15 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                 o[bl] *= a.scale * eg[16 * bl + n];
 #pragma unroll
                 for (int c = 0; c < (bl + 1) / 2; ++c) {
-                    uint4 f[PL];
+                    uint4 f[3];
 #pragma unroll
-                    for (int l = 0; l < PL; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
-                    o[bl] = gd_mul_t<PL - 1>(f, ul[c], o[bl]);
+                    for (int l = 0; l < 3; ++l) f[l] = *(const uint4*)Pf[(bl + 1) * (bl + 1) / 4 + c][l][lane];
+                    o[bl] = gd_mul_t(f, ul[c], o[bl]);
                 }
                 if (!(bl & 1)) {
-                    uint2 f[PL];
+                    uint2 f[3];
 #pragma unroll
-                    for (int l = 0; l < PL; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
+                    for (int l = 0; l < 3; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
                     o[bl] = gd_mul16_t(f, ul[bl / 2], o[bl]);
                 }
                 if (hurt)
@@ -630,7 +630,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                         const uint2 f0 = gd_column(p), f1 = gd_column(p + 16 * LDK);
                         f[l] = make_uint4(f0.x, f0.y, f1.x, f1.y);
                     }
-                    S[c] = gd_mul<2>(f, wl, S[c]);
+                    S[c] = gd_mul(f, wl, S[c]);
                 }
         }
         if (hurt && bad < C) {

@@ -523,6 +523,28 @@ def test_large_and_small_values_keep_their_precision(dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_outputs_that_are_small_differences_of_large_terms(dtype):
+    """A key that is written again takes back what it held: o = q S + P u, here (q = k, |k| = 1, beta = 1, no decay, scale 1: o = v) of terms `size` times
+    the result.  An output takes Dk + 64 sums for these two and, through P (rows of norm sqrt(2) at most), Dk + 64 + 16 for u: 128 + 2 * 144 = 416
+    roundings, each of at most half a step of fp32 of a partial sum, whose rms is `size`; signs are random, so the rms error is at
+    most sqrt(416) u size, and the result's own rounding half a step / sqrt(3).  Terms of 16 bits would be off by 2^-16 of theirs, 4 to 5 times that."""
+    B, T, H, D, size = 2, 64, 4, 64, 4096.0
+    gen = torch.Generator().manual_seed(21)
+    k = (torch.randint(0, 2, (B, T, H, D), generator=gen) * 2 - 1).to(dtype).cuda() / 8          # exact in every type, and so is its norm
+    v = torch.randn(B, T, H, D, generator=gen).to(dtype).cuda()
+    g, beta = torch.zeros(B, T, H, device="cuda"), torch.ones(B, T, H, device="cuda")
+    state = size * torch.randn(B, H, D, D, generator=gen).cuda()
+    ref, _ = delta_rule(k, k, v, g, beta, state=state, scale=1.0)
+    assert float((ref - v.double().cpu()).abs().max()) < 1e-9
+    out, _ = operators.gated_delta(k, k, v, g, beta, state=state, scale=1.0)
+    off = float((out.double().cpu() - ref).square().mean().sqrt())
+    own = HALF_STEP[dtype] / math.sqrt(3) * float(ref.square().mean().sqrt())
+    bound = math.hypot(math.sqrt(416) * U * size, own)
+    assert off <= bound, f"rms {off:.3g}, {off / bound:.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("T, lens, Hk, Hv, Dk, Dv", [(1200, None, 1, 2, 64, 64), (2000, (2000, 777), 1, 1, 16, 40), (1500, (0, 1500), 2, 2, 128, 128), (900, (64, 899), 1, 2, 48, 20),
                                                      (1030, None, 1, 1, 100, 100)])
 def test_few_long_clips_are_cut_into_segments(T, lens, Hk, Hv, Dk, Dv, dtype):
