@@ -22,7 +22,7 @@ struct GatedDeltaArgs {
     int sorted;                       // clips: the longest first (batch: at most GD_RANKED)
     int whole, even;                  // k and q can be read in pieces of eight values (hops: v in pieces of four too), out written in pieces of four
     int segments, seg;                // clips: how many pieces a clip is cut into, and their frames
-    float* starts;                    // [segments][B Hv][Dk][Dv]: the states that segments 1 .. start with; before they are joined, what each adds
+    float* starts;                    // [segments][B Hv][Dk][Dv]: the states that segments start with (the first: if there is a state_in); before they are joined, what each adds
     float* moves;                     // [segments][B Hv][Dk][Dk]: segment i's effect on the state before it, i = 1 .. segments - 2
     float scale;
 };
@@ -215,7 +215,8 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
 // is written again, Q S and P u cancel, and what counts is 2^-24 of the terms, not the rounding of the result.
 //
 // Where there are fewer heads than the chip holds workgroups, the frames are cut into segments.  A segment's effect on the state before it is
-// linear, S -> M S + N: MOVE runs a segment from S = 0 with its v (N) and from the unit matrix without (M, Dk columns more), no outputs;
+// linear, S -> M S + N: MOVE runs a segment from S = 0 with its v (N; the first one from the clip's state) and from the unit matrix without (M, Dk
+// columns more), no outputs;
 // gated_delta_join_kernel then walks the segments (N becomes the state that the next one starts with), and the segments run as
 // clips of their own.  About two and a half times the work, over `segments` times the workgroups.
 //
@@ -372,7 +373,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
     const long vb = (long)b * a.vs[0] + (long)h * a.vs[2], ob = (long)b * a.os[0] + (long)h * a.os[2];
     const long gb = (long)b * a.gs[0] + (long)h * a.gs[2], bb = (long)b * a.bs[0] + (long)h * a.bs[2];
     const long sb = head * a.Dk * a.Dv + col;
-    const float* from = sg == 0 ? a.state_in : MOVE ? nullptr : a.starts + (long)sg * heads * a.Dk * a.Dv;
+    // the last segment may write the final state over state_in: the first one starts from the copy of it that the join, the launch before, has left
+    const float* from = MOVE ? (sg == 0 ? a.state_in : nullptr) : sg > 0 || (a.segments > 1 && a.state_in) ? a.starts + (long)sg * heads * a.Dk * a.Dv : a.state_in;
     const unsigned vstep = (unsigned)a.vs[1] * E, ostep = (unsigned)a.os[1] * E;
     const unsigned voff = cin && !eye ? 4 * q * vstep + col * E : GD_OUT;
     const int ocol = col - n + 4 * q;                      // out: row n of a block, four columns
@@ -652,7 +654,8 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
 }
 
 // The segments' states one after the other, S <- M S + N on the fp32 matrix instruction: a workgroup is 16 columns of a head, wave c its rows
-// 16 c .. 16 c + 15; the state goes round through LDS.
+// 16 c .. 16 c + 15; the state goes round through LDS.  starts[0] becomes a copy of state_in (in this kernel: in MOVE its stores stood in front
+// of the first chunk's loads, 16 clips of 1003 frames, 4 heads of 64, fp32, 3 us).
 template <int DKP>
 __global__ __launch_bounds__(4 * DKP) void gated_delta_join_kernel(GatedDeltaArgs a, long heads) {
     constexpr int NB = DKP / 16;
@@ -681,8 +684,11 @@ __global__ __launch_bounds__(4 * DKP) void gated_delta_join_kernel(GatedDeltaArg
                 for (int i = 0; i < 4; ++i) x[c][i] = 16 * c + 4 * q + i < a.Dk ? mv[(long)s * mstep + 16 * c + 4 * q + i] : 0.f;
     };
     // segment s's matrix and the next one's addition are on their way while segment s - 1 is joined
-    float x[4], nx[4];
+    float x[4], nx[4], s0[4] = {0.f, 0.f, 0.f, 0.f};
     f32x4 m[NB];
+    if (a.state_in)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s0[i] = cin && row + i < a.Dk ? a.state_in[sb + (long)(row + i) * a.Dv] : 0.f;
     piece(1, x);
     if (a.segments > 2) { matrix(1, m); piece(2, nx); }
     for (int s = 1; s + 1 < a.segments; ++s) {
@@ -706,4 +712,8 @@ __global__ __launch_bounds__(4 * DKP) void gated_delta_join_kernel(GatedDeltaArg
             if (cin && row + i < a.Dk) a.starts[(long)(s + 1) * step + sb + (long)(row + i) * a.Dv] = y[0][i];
         }
     }
+    if (a.state_in)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (cin && row + i < a.Dk) a.starts[sb + (long)(row + i) * a.Dv] = s0[i];
 }

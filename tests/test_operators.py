@@ -572,6 +572,23 @@ def test_few_long_clips_are_cut_into_segments(T, lens, Hk, Hv, Dk, Dv, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("B, T, lens, Hk, Hv, Dk, Dv", [(1, 1200, None, 1, 2, 64, 64), (3, 1500, (0, 200, 1500), 1, 2, 32, 40), (2, 1030, (1, 700), 2, 2, 128, 128),
+                                                        (3, 900, (900, 0, 64), 1, 1, 100, 20)])
+def test_segments_update_a_state_in_place(B, T, lens, Hk, Hv, Dk, Dv, dtype):
+    """The first segment starts from the state that the last one, which has no frames in a short clip, writes over: the same bits as with two states."""
+    x = inputs(B, T, Hk, Hv, Dk, Dv, dtype, seed=T, g_std=3.0)
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    state = 0.5 * torch.randn(B, Hv, Dk, Dv, generator=torch.Generator().manual_seed(1)).cuda()
+    want, wend = operators.gated_delta(*x, state=state, lengths=lengths)
+    near(wend, delta_rule(*x, state=state, lengths=lengths)[1], tol(T, Dk))
+    for _ in range(5):
+        s = state.clone()
+        out, end = operators.gated_delta(*x, state=s, lengths=lengths, state_out=s)
+        assert end is s and torch.equal(out, want) and torch.equal(s, wend)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("Dv", [20, 60, 100])
 @pytest.mark.parametrize("Dk", [20, 50, 100])
 def test_long_clips_of_every_size(Dk, Dv, dtype):
