@@ -57,6 +57,7 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
         for (int i = 0; i < 3; ++i) if (s[i] < 0) return set_err(DPDF_E_INVALID, "gated delta rule: negative stride");
     const long n = B * Hv * Dk * Dv * 4;
     const OpSpan si = {(const char*)x.state_in, (const char*)x.state_in + (x.state_in ? n : 0)}, so = {(const char*)x.state_out, (const char*)x.state_out + (x.state_out ? n : 0)};
+    const OpSpan len = {(const char*)x.lengths, (const char*)x.lengths + (x.lengths ? B * 4 : 0)}, act = {(const char*)x.active, (const char*)x.active + (x.active ? B : 0)};
     if (B && T) {
         if (!x.q || !x.k || !x.v || !x.g || !x.beta || !x.out) return set_err(DPDF_E_INVALID, "null argument");
         if (!op_aligned(x.q, e) || !op_aligned(x.k, e) || !op_aligned(x.v, e) || !op_aligned(x.out, e) || !op_aligned(x.g, ge) || !op_aligned(x.beta, ge))
@@ -67,7 +68,9 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
                               op_span(x.g, x.g_stride, vd, 3, 1, ge), op_span(x.beta, x.beta_stride, vd, 3, 1, ge)};
         for (const OpSpan& i : in) if (op_meet(o, i) || op_meet(so, i)) return set_err(DPDF_E_INVALID, "gated delta rule: an output overlaps an input");
         if (op_meet(o, si) || op_meet(o, so)) return set_err(DPDF_E_INVALID, "gated delta rule: out overlaps a state");
+        if (op_meet(o, len) || op_meet(o, act)) return set_err(DPDF_E_INVALID, "gated delta rule: an output overlaps an input");
     }
+    if (op_meet(so, len) || op_meet(so, act)) return set_err(DPDF_E_INVALID, "gated delta rule: an output overlaps an input");
     if (x.state_in != x.state_out && op_meet(si, so)) return set_err(DPDF_E_INVALID, "gated delta rule: the states overlap in part");
     if (!op_aligned(x.state_in, 4) || !op_aligned(x.state_out, 4) || !op_aligned(x.lengths, 4)) return set_err(DPDF_E_INVALID, "gated delta rule: a pointer is not aligned to its type");
     a.q = x.q; a.k = x.k; a.v = x.v; a.g = x.g; a.beta = x.beta; a.out = x.out;
@@ -208,9 +211,10 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
             a.seg = (int)(each * chunk); a.segments = (int)((chunks + each - 1) / each);
             const OpSpan ws = {(const char*)workspace, (const char*)workspace + gd_workspace(a, heads, a.segments)};
             const long B = args->batch, T = args->frames, kd[3] = {B, T, a.Hk}, vd[3] = {B, T, a.Hv}, ge = op_bytes(args->gate_dtype), state = heads * a.Dk * a.Dv * 4;
-            const OpSpan other[8] = {op_span(a.q, a.qs, kd, 3, a.Dk, e), op_span(a.k, a.ks, kd, 3, a.Dk, e), op_span(a.v, a.vs, vd, 3, a.Dv, e), op_span(a.out, a.os, vd, 3, a.Dv, e),
+            const OpSpan other[9] = {op_span(a.q, a.qs, kd, 3, a.Dk, e), op_span(a.k, a.ks, kd, 3, a.Dk, e), op_span(a.v, a.vs, vd, 3, a.Dv, e), op_span(a.out, a.os, vd, 3, a.Dv, e),
                                      op_span(a.g, a.gs, vd, 3, 1, ge), op_span(a.beta, a.bs, vd, 3, 1, ge),
-                                     {(const char*)a.state_in, (const char*)a.state_in + (a.state_in ? state : 0)}, {(const char*)a.state_out, (const char*)a.state_out + (a.state_out ? state : 0)}};
+                                     {(const char*)a.state_in, (const char*)a.state_in + (a.state_in ? state : 0)}, {(const char*)a.state_out, (const char*)a.state_out + (a.state_out ? state : 0)},
+                                     {(const char*)a.lengths, (const char*)a.lengths + (a.lengths ? B * 4 : 0)}};
             for (const OpSpan& o : other) if (op_meet(ws, o)) return set_err(DPDF_E_INVALID, "gated delta rule: the workspace overlaps a tensor");
             a.starts = (float*)workspace; a.moves = a.starts + (size_t)a.segments * heads * a.Dk * a.Dv;
         }

@@ -166,6 +166,15 @@ def test_gated_delta_step_refusals_and_empty_calls():
         assert _c_gated()[0] == -2 and _c_gated(step=True)[0] == -2        # no GPU: a failure, nothing computed elsewhere
 
 
+@pytest.mark.parametrize("change", [
+    dict(lengths=0x6000000), dict(lengths=0x6000000 - 4), dict(lengths=0x7000000), dict(lengths=0x7000000 + 2 * 4 * 16 * 8 * 4 - 4), dict(frames=0, lengths=0x7000000),
+    dict(step=True, active=0x6000001), dict(step=True, active=0x7000000 + 2 * 4 * 16 * 8 * 4 - 1), dict(step=True, active=0x7000000 - 1),
+])
+def test_lengths_and_masks_in_an_outputs_memory_are_refused(change):
+    rc, msg = _c_gated(**change)
+    assert rc == -1 and "overlaps an input" in msg, (rc, msg)
+
+
 def _c_w4(**change):
     v = dict(dtype=1, scale_dtype=1, rows=2, in_dim=100, out_dim=6, group=32, x=0x1000000, x_stride=100, codes=0x2000000, codes_pitch=50,
              scales=0x3000000, scales_stride=4, zeros=0x4000000, zeros_pitch=4, bias=0x5000000, out=0x6000000, out_stride=6)
@@ -568,6 +577,25 @@ def test_few_long_clips_are_cut_into_segments(T, lens, Hk, Hv, Dk, Dv, dtype):
     assert L.dpdf_gated_delta(0, ctypes.addressof(a), None, 0, torch.cuda.current_stream().cuda_stream) == 0
     near(out1, ref, tol(T, Dk), HALF_STEP[dtype], TINY[dtype])
     near(end1, rend, tol(T, Dk))
+
+
+@pytest.mark.gpu
+def test_a_workspace_over_the_lengths_is_refused():
+    B, T, H, D = 1, 1200, 1, 64
+    x = inputs(B, T, H, H, D, D, F32)
+    out, end = torch.zeros(B, T, H, D, device="cuda"), torch.zeros(B, H, D, D, device="cuda")
+    room = torch.zeros(1 << 20, dtype=torch.int32, device="cuda")
+    strides = [(T * H * D, H * D, D)] * 3 + [(T * H, H, 1)] * 2 + [(T * H * D, H * D, D)]
+    L = backend.load_library()
+    for at in (0, 5):
+        lengths = room[at:at + B]
+        lengths.fill_(T)
+        a = operators._GatedDeltaArgs(0, 0, B, T, H, H, D, D, 1.0, *[t.data_ptr() for t in x], out.data_ptr(), *strides, None, end.data_ptr(), lengths.data_ptr(), None)
+        assert 0 < L.dpdf_gated_delta_workspace(0, ctypes.addressof(a)) <= 4 * room.numel()
+        assert L.dpdf_gated_delta(0, ctypes.addressof(a), room.data_ptr(), 4 * room.numel(), torch.cuda.current_stream().cuda_stream) == -1
+        assert "workspace overlaps" in L.dpdf_last_error().decode()
+    torch.cuda.synchronize()
+    assert bool((out == 0).all()) and bool((end == 0).all())
 
 
 @pytest.mark.gpu
