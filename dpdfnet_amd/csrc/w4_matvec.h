@@ -17,11 +17,11 @@ struct W4Args {
 };
 
 // Sixteen outputs at a time on the matrix units: x is the left operand (its rows the tile's rows, so that one row costs what sixteen do: the
-// time is that of reading the codes), the weights are the right one.  A nibble becomes a 16-bit float in two instructions, a shift and an
-// and-or, as 16 + code: the four bits are the significand of a number in [16, 32), exactly, in bf16 and in fp16.  The offset goes out with the
-// zero, for a group: sum x (code - zero) = sum x (16 + code) - (16 + zero) sum x, sum x from one more product, with ones.  Products are exact;
-// sums are fp32 and up to (16 + 15) / |code - zero| (five times on average) the magnitude they end with, which costs about two bits of 24.
-// Nibble t and t + 4 of a word come out together, so x is brought into the order 0 4 1 5 2 6 3 7.  fp32 rows go in as three bf16 limbs
+// time is that of reading the codes), the weights are the right one, as code - zero, which both 16-bit types hold exactly: a term whose code is
+// the zero is 0, products are exact, and the sums' roundings go by the terms alone.  A group's sum is taken before its scale.
+// Four codes to a word of bytes, e = 128 + zero - code: from 128 on that is a sign and |code - zero|, below it 128 - e is, and a byte of a
+// sign and 0 .. 15 is that many steps of 2^-9 as an 8-bit float (e4m3, whose steps are even up to there): 17 instructions for eight weights.
+// Codes 0 2 4 6 and 1 3 5 7 of a word come out together, so x is brought into that order.  fp32 rows go in as three bf16 limbs
 // (exact, see gru_limb.h), three products each.
 //
 // A workgroup is 16 NT outputs; each wave takes a run of blocks of 128 inputs, two blocks in flight, and the waves' sums meet in LDS in a fixed
@@ -31,7 +31,9 @@ struct W4Args {
 // LDS as fp32: read block by block, 2 bytes of 16 rows at a time, they cost more than the codes (8192 x 32768: 25 of 72 us).
 //
 // Bound: reading the codes; what keeps it from a plain read's rate (24.6 us for the codes of 8192 x 32768, 5.5 TB/s) is the traffic beside them,
-// x about 7 us and scales 5.  8192 x 32768, eight rows of bf16: 44 us, 3.2 TB/s; 4096 x 16384, one row: 11.7 us, 3.0 TB/s; 4096 x 4096, 16 rows: 8.1 us.
+// x about 7 us and scales 5, and the instructions for code - zero (16 + code, with (16 + zero) sum x taken off a group's sum, took 8 for eight weights and
+// 44 us, but its error went by 16 to 31 times |x|).  8192 x 32768, eight rows of bf16: 47 us, 3.0 TB/s; 4096 x 16384, one row: 12.3 us, 2.8 TB/s; 4096 x 4096, 16 rows:
+// 8.0 us.
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 template <typename T> struct W4X;                 // eight inputs of a row as a left operand: LIMBS fragments
@@ -39,14 +41,20 @@ template <> struct W4X<__hip_bfloat16> { enum { LIMBS = 1 }; };
 template <> struct W4X<__half> { enum { LIMBS = 1 }; };
 template <> struct W4X<float> { enum { LIMBS = 3 }; };
 
-// the eight weights of a word; mask and base (w4_mask, w4_base) come in registers of which one instruction can read both
-template <typename T> __device__ __forceinline__ unsigned w4_mask() { unsigned m = __is_same(T, __half) ? 0x03c003c0u : 0x00780078u; asm("" : "+v"(m)); return m; }
-template <typename T> __device__ __forceinline__ unsigned w4_base() { unsigned b = __is_same(T, __half) ? 0x4c004c00u : 0x41804180u; asm("" : "+s"(b)); return b; }
-template <typename T> __device__ __forceinline__ uint4 w4_weights(unsigned w, unsigned mask, unsigned base) {
-    if constexpr (__is_same(T, __half)) return make_uint4(((w << 6) & mask) | base, ((w << 2) & mask) | base, ((w >> 2) & mask) | base, ((w >> 6) & mask) | base);
-    else return make_uint4(((w << 3) & mask) | base, ((w >> 1) & mask) | base, ((w >> 5) & mask) | base, ((w >> 9) & mask) | base);
+// code - zero of four codes in bytes, as signs and magnitudes; zero: 128 + the zero in every byte
+__device__ __forceinline__ unsigned w4_signed(unsigned codes, unsigned zero) {
+    const unsigned e = zero - codes, over = ~e & 0x80808080u, one = over >> 7;      // over: where the code is more than the zero
+    return (e ^ (over - one)) + one;
 }
-template <typename T> __device__ __forceinline__ unsigned w4_one() { return __is_same(T, __half) ? 0x3c003c00u : 0x3f803f80u; }
+template <typename T> __device__ __forceinline__ uint4 w4_weights(unsigned w, unsigned zero) {
+    const unsigned a = w4_signed(w & 0x0f0f0f0fu, zero), b = w4_signed(w >> 4 & 0x0f0f0f0fu, zero);
+    if constexpr (__is_same(T, __half))
+        return make_uint4(__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 512.f, false)), __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 512.f, true)),
+                          __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 512.f, false)), __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 512.f, true)));
+    else
+        return make_uint4(__builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.f, false)), __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.f, true)),
+                          __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.f, false)), __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.f, true)));
+}
 template <typename T> __device__ __forceinline__ f32x4 w4_mfma(const uint4& a, const uint4& b, f32x4 c) {
     if constexpr (__is_same(T, __half)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
     else return mfma_bf16(a, b, c);
@@ -56,13 +64,13 @@ template <typename T> struct W4Eight { T v[8]; };
 template <typename T> __device__ __forceinline__ void w4_limbs(const W4Eight<T>& x, uint4 (&f)[W4X<T>::LIMBS]) {
     if constexpr (sizeof(T) == 2) {
         const uint4 v = __builtin_bit_cast(uint4, x);
-        f[0] = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
-                          __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
+        f[0] = make_uint4(__builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x05040100u),
+                          __builtin_amdgcn_perm(v.y, v.x, 0x07060302u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u));
     } else {
         const float* h = x.v;
         uint2 a0, a1, a2, b0, b1, b2;
-        split3(make_float4(h[0], h[4], h[1], h[5]), a0, a1, a2);
-        split3(make_float4(h[2], h[6], h[3], h[7]), b0, b1, b2);
+        split3(make_float4(h[0], h[2], h[4], h[6]), a0, a1, a2);
+        split3(make_float4(h[1], h[3], h[5], h[7]), b0, b1, b2);
         f[0] = make_uint4(a0.x, a0.y, b0.x, b0.y); f[1] = make_uint4(a1.x, a1.y, b1.x, b1.y); f[2] = make_uint4(a2.x, a2.y, b2.x, b2.y);
     }
 }
@@ -78,7 +86,7 @@ template <typename T> struct W4Inputs { W4Eight<T> v[4]; };
 template <typename T, typename G, int R, int NT>
 __global__ __launch_bounds__(64 * W4_WAVES) void w4_matvec_kernel(W4Args a) {
     constexpr int L = W4X<T>::LIMBS, SUB = 4 / R;       // SUB: groups that a block is cut into
-    typedef float2 Scales[4 * SUB][16 * NT];            // of four blocks: scale, -16 - zero
+    typedef float2 Scales[4 * SUB][16 * NT];            // of four blocks: scale, 128 + zero in every byte
     typedef float Sums[NT][16][17];
     constexpr int ROOM = sizeof(Scales) > sizeof(Sums) ? sizeof(Scales) : sizeof(Sums);
     __shared__ __attribute__((aligned(16))) unsigned char room[W4_WAVES][ROOM];
@@ -105,14 +113,14 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_matvec_kernel(W4Args a) {
         const float first = a.bias && w == 0 ? gd_load<T>(a.bias, o) : 0.f;      // the bias goes into the first wave's sums
         y[t] = (f32x4){first, first, first, first};
     }
-    const unsigned per32 = (unsigned)a.group / 32, mask = w4_mask<T>(), base = w4_base<T>();
+    const unsigned per32 = (unsigned)a.group / 32;
     Scales& sc = *(Scales*)room[w];
     auto put = [&](const G (&s)[NT][SUB], const unsigned char (&z)[NT][SUB]) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) sc[SUB * q + u][16 * t + n] = make_float2(gd_load<G>(&s[t][u], 0), zeros ? -16.f - (float)z[t][u] : -24.f);
+            for (int u = 0; u < SUB; ++u) sc[SUB * q + u][16 * t + n] = make_float2(gd_load<G>(&s[t][u], 0), __builtin_bit_cast(float, zeros ? 0x01010101u * (128u + z[t][u]) : 0x88888888u));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
     // one block, the j-th of the four whose scales are in LDS
@@ -124,31 +132,27 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_matvec_kernel(W4Args a) {
             for (int r = 0; r < 4; ++r) c[t][r] = codes.v[t][r];
             w4_swap32(c[t][0], c[t][2]); w4_swap32(c[t][1], c[t][3]); w4_swap16(c[t][0], c[t][1]); w4_swap16(c[t][2], c[t][3]);
         }
-        const unsigned o1 = w4_one<T>();
 #pragma unroll
         for (int u = 0; u < SUB; ++u) {
-            f32x4 acc[NT], one = {0.f, 0.f, 0.f, 0.f};
+            f32x4 acc[NT];
+            float2 s[NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) acc[t] = one;
+            for (int t = 0; t < NT; ++t) { acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f}; s[t] = sc[SUB * j + u][16 * t + n]; }
 #pragma unroll
             for (int r = R * u; r < R * (u + 1); ++r) {
                 uint4 f[L];
                 w4_limbs<T>(x.v[r], f);
 #pragma unroll
-                for (int l = L - 1; l >= 0; --l) one = w4_mfma<T>(f[l], make_uint4(o1, o1, o1, o1), one);
-#pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const uint4 wt = w4_weights<T>(c[t][r], mask, base);
+                    const uint4 wt = w4_weights<T>(c[t][r], __builtin_bit_cast(unsigned, s[t].y));
 #pragma unroll
                     for (int l = L - 1; l >= 0; --l) acc[t] = w4_mfma<T>(f[l], wt, acc[t]);
                 }
             }
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float2 s = sc[SUB * j + u][16 * t + n];
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[t][i] = __builtin_fmaf(s.x, __builtin_fmaf(s.y, one[i], acc[t][i]), y[t][i]);
-            }
+                for (int i = 0; i < 4; ++i) y[t][i] = __builtin_fmaf(s[t].x, acc[t][i], y[t][i]);
         }
     };
     // the last wave takes what is left of the inputs, and nothing else where the others have no more to do for it

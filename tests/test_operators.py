@@ -812,6 +812,55 @@ def test_w4_rows_are_independent_and_repeat(dtype, M):
     assert torch.equal(got[:, keep], y[:, keep]) and not bool(torch.isfinite(got[:, 5]).any())
 
 
+def near_sparse_layer(y, x, codes, scales, z, group, dtype):
+    """Weights near their zero: a term whose code is the zero is 0 and adds nothing, the n others of an output are at most three products each (fp32 rows
+    are three limbs) with one sum each, and a scale and a sum per group: 8 deviations of sqrt(5 n) roundings of the terms' magnitudes."""
+    ref, mag = w4_layer(x, codes, scales, z, None, group)
+    k = torch.arange(x.shape[-1])
+    code = (codes.cpu()[:, k // 2].int() >> (4 * (k % 2))) & 15
+    n = (code != (8 if z is None else z.cpu()[:, k // group].int())).sum(1).double()
+    bound = 8 * (5 * n).sqrt() * U * mag + HALF_STEP[dtype] * ref.abs() * 1.01 + TINY[dtype] * (n > 0)
+    off = (y.double().cpu() - ref).abs()
+    assert bool((off <= bound).all()), f"worst {float((off / bound.clamp_min(1e-300)).max()):.3g} of the bound"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("M, K, N, group", [(1, 4096, 48, 64), (5, 1000, 40, 32), (16, 2048, 40, 128), (3, 301, 20, 96)])
+@pytest.mark.parametrize("zero", [None, 0, 3, 11, 15])
+def test_w4_weights_near_their_zero(M, K, N, group, zero, dtype):
+    """Rows of nothing but zeros (0, exactly), of one weight, of a few, of weights close around the zero."""
+    gen = torch.Generator().manual_seed(K + (zero or 0))
+    x, _, scales, _, bias = layer(M, K, N, group, dtype, False, seed=K)
+    at = 8 if zero is None else zero
+    code = torch.full((N, K + K % 2), at)
+    for n in range(N):
+        if n % 4 == 1:
+            code[n, torch.randint(0, K, (1,), generator=gen)] = (at + 1 + n) % 16
+        elif n % 4 == 2:
+            code[n, torch.randint(0, K, (7,), generator=gen)] = torch.randint(0, 16, (7,), generator=gen)
+        elif n % 4 == 3:
+            code[n] = (at + (0.7 * torch.randn(K + K % 2, generator=gen)).round().long()).clamp(0, 15)
+    codes = (code[:, ::2] | code[:, 1::2] << 4).to(torch.uint8).cuda()
+    z = None if zero is None else torch.full(scales.shape, zero, dtype=torch.uint8, device="cuda")
+    y = operators.w4_matvec(x, codes, scales, zeros=z, group=group)
+    near_sparse_layer(y, x, codes, scales, z, group, dtype)
+    assert bool((y[:, ::4] == 0).all())
+    yb = operators.w4_matvec(x, codes, scales, zeros=z, bias=bias, group=group)
+    assert torch.equal(yb[:, ::4], bias[::4].expand(M, -1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_w4_large_inputs_are_not_taken_out_of_range(dtype):
+    """|x| of 2e37, two in a row: their products with code - zero, 8 at most, stay below 3.4e38, and so does their sum."""
+    x, codes, scales, _, _ = layer(4, 640, 40, 64, dtype, False, seed=5)
+    keep = torch.zeros_like(x)
+    keep[:, [3, 630]] = torch.tensor([1.0, -1.0], device="cuda", dtype=dtype)
+    x = keep * 2e37
+    near_sparse_layer(operators.w4_matvec(x, codes, scales), x, codes, scales, None, 64, dtype)
+
+
 @pytest.mark.gpu
 def test_w4_empty_batch_and_far_offsets():
     x, codes, scales, z, bias = layer(3, 128, 40, 64, F16, False)
