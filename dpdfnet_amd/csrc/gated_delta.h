@@ -203,7 +203,7 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
 // ---------------------------------------------------------------------------------------------------------------------------------------
 // Clips: chunks of C frames.  With gamma = the running sum of g inside the chunk, d_ij = exp(gamma_i - gamma_j) and S the state before it,
 //     A_ij = beta_i d_ij k_i.k_j (j < i),   (I + A) u = beta (v - exp(gamma) (K S)),
-//     O = scale exp(gamma) (Q S) + P u,   P_ij = scale d_ij q_i.k_j (j <= i),   S <- exp(gamma_C) S + K^T (exp(gamma_C - gamma) u):
+//     O = scale (exp(gamma) (Q S) + P u),   P_ij = d_ij q_i.k_j (j <= i),   S <- exp(gamma_C) S + K^T (exp(gamma_C - gamma) u):
 // matrix products, and 16 dependent steps for the inverses of the 16 x 16 diagonal blocks of I + A where the definition has C.
 //
 // A workgroup is one head and 16 NW columns: wave w owns 16 columns of S, u and O in the matrix units' result layout (row 4 q + i, column n),
@@ -449,8 +449,22 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
         if (w == 0) {
             if (lane >= m) { ng = 0.f; nbt = 0.f; }
             if (!(ng < __builtin_inff()) || !gd_finite(nbt)) { atomicMin(&kbad[par], lane); ng = 0.f; nbt = 0.f; }
-            // in powers of two; exp(-128) is 0 in fp32 already: -inf, a reset, comes without inf - inf
-            const double s = gd_scan((ng < -128.f ? -128.0 : (double)ng) * 1.4426950408889634);
+            // in powers of two; -inf, a reset, comes as -8192, without inf - inf: far below what growth inside a chunk, which is held to 2^127, brings back
+            auto sum = [&] { return gd_scan((ng < -8192.f ? -8192.0 : (double)ng) * 1.4426950408889634); };
+            double s = sum();
+            if (__any(ng > 0.f)) {
+                // growth since the chunk's beginning or a frame of it: from the first frame on that has more than fp32 holds, NaN, and finite operands
+                float low = fminf((float)s, 0.f);
+#pragma unroll
+                for (int o = 1; o < 64; o <<= 1) low = fminf(low, __shfl_up(low, o));         // lanes below o get their own
+                const unsigned long over = __ballot((float)s - low > 127.f);
+                if (over) {
+                    const int at = __builtin_ctzl(over);
+                    if (lane == 0) atomicMin(&kbad[par], at);
+                    if (lane >= at) { ng = 0.f; nbt = 0.f; }
+                    s = sum();
+                }
+            }
             const double last = __shfl(s, C - 1);
             if (lane < C) {
                 const float hi = (float)s;
@@ -496,7 +510,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             for (int i = 0; i < 4; ++i) {
                 const float d = __builtin_amdgcn_exp2f((gr.x - gh[i]) + (gr.y - gl[i]));
                 xa[i] *= br * d;
-                xp[i] *= a.scale * d;
+                xp[i] *= d;
             }
             if (bi == bj) {
 #pragma unroll
@@ -600,7 +614,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
             u = mfma16(t.x, z[0], u); u = mfma16(t.y, z[1], u); u = mfma16(t.z, z[2], u); u = mfma16(t.w, z[3], u);
             gd_split(u, ul[bl / 2], bl & 1);
             if constexpr (!MOVE) {
-                o[bl] *= a.scale * eg[16 * bl + n];
+                o[bl] *= eg[16 * bl + n];
 #pragma unroll
                 for (int c = 0; c < (bl + 1) / 2; ++c) {
                     uint4 f[3];
@@ -614,6 +628,7 @@ __global__ __launch_bounds__(64 * NW, 2) void gated_delta_clip_kernel(GatedDelta
                     for (int l = 0; l < 3; ++l) f[l] = Pf[(bl + 1) * (bl + 1) / 4 + bl / 2][l][lane][0];
                     o[bl] = gd_mul16_t(f, ul[bl / 2], o[bl]);
                 }
+                o[bl] *= a.scale;                          // not a factor of P: d alone may be near fp32's end
                 if (hurt)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)

@@ -232,7 +232,8 @@ typedef struct dpdf_gated_delta_args {
 
 /* Whole clips, in chunks of 32 or 64 frames.  Frames behind a clip's length are neither read nor written; state_out is the state after its last
  * frame (a clip of length 0: the state it came with).  A non-finite k, g (but -inf) or beta makes the outputs of its head from its frame
- * on, and its state, NaN, a non-finite v those of its column, a non-finite q those of its frame; nothing earlier and no other head.
+ * on, and its state, NaN, a non-finite v those of its column, a non-finite q those of its frame; nothing earlier and no other head.  Where positive g
+ * add up to more than 88 inside a chunk (exp of it leaves fp32), the frame where they do counts as one of a non-finite g.
  *
  * Few heads over many frames are cut into segments that run side by side, given a workspace for the segments' states:
  * dpdf_gated_delta_workspace() bytes on the device, aligned to 16, the call's alone until it has run; 0 where there is nothing to cut.

@@ -315,6 +315,49 @@ def test_gates_of_the_values_type(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("drop, up", [(-140.0, 43.0), (-200.0, 75.0)])
+def test_growth_behind_a_reset_brings_nothing_back(drop, up, dtype):
+    """g = -inf empties the state whatever follows; a large negative g and growth after it are what their sum is.  Without writes (beta = 0) the
+    outputs are exp(sum of g) S0^T q: 0 behind the reset, exp(-140 + 86) of it for the second head.  exp's argument, -78 in powers of two, is off by
+    half a step of fp32 there (2^-18), the result by as much, the sums by tol().  Growth by 150 in two frames is more than fp32
+    holds: from the second of them on clips give NaN, and everything before is as it was."""
+    T, D, scale = 40, 32, 1e20 if dtype != F16 else 1.0
+    q, k, v, g, beta = inputs(1, T, 1, 3, D, D, dtype, seed=31)
+    g, beta = torch.zeros_like(g), torch.zeros_like(beta)
+    for h, down in enumerate((-math.inf, drop, -1000.0)):
+        g[:, 3, h], g[:, 5:7, h] = down, up
+    state = torch.randn(1, 3, D, D, generator=torch.Generator().manual_seed(1)).cuda()
+    out, end = operators.gated_delta(q, k, v, g, beta, state=state, scale=scale)
+    ref, rend = delta_rule(q, k, v, g, beta, state=state, scale=scale)
+    n = 6 if 2 * up > 88 else T
+    near(out[:, :3], ref[:, :3], tol(T, D), HALF_STEP[dtype], TINY[dtype])
+    assert bool((out[:, 3:n, [0, 2]] == 0).all())
+    if n < T:
+        assert bool(out[:, n:].isnan().all()) and bool(end.isnan().all())
+    else:
+        assert bool((end[:, [0, 2]] == 0).all())
+        near(out[:, 7:, 1], ref[:, 7:, 1], tol(T, D) + 2.0 ** -16, HALF_STEP[dtype], TINY[dtype])
+        near(end[:, 1], rend[:, 1], tol(T, D) + 2.0 ** -16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("T, at", [(90, 20), (90, 70), (1200, 700)])
+def test_growth_beyond_fp32_spares_what_is_before_it(T, at, dtype):
+    """exp(g) of one frame, or of several together, outside fp32: NaN from there on, the frames before bit for bit, and the other head."""
+    x = inputs(1, T, 1, 2, 32, 32, dtype, seed=T)
+    clean, cend = operators.gated_delta(*x)
+    for grow in ([100.0], [40.0, 40.0, 40.0]):
+        g, first = x[3].clone(), at + 1 - len(grow)
+        g[0, first:at + 1, 0] = torch.tensor(grow, device="cuda")
+        out, end = operators.gated_delta(*x[:3], g, x[4])
+        assert torch.equal(out[:, :first], clean[:, :first]) and torch.equal(out[:, :, 1], clean[:, :, 1]) and torch.equal(end[:, 1], cend[:, 1])
+        assert dtype == F16 or bool(out[:, :at, 0].isfinite().all())              # exp(80) is in range, but not of fp16
+        assert bool(out[:, at:, 0].isnan().all()) and bool(end[:, 0].isnan().all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("D", [64, 128])
 def test_hard_gates_and_keys(dtype, D):
