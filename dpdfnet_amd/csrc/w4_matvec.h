@@ -284,6 +284,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_matvec_kernel(W4Args a) {
 
 // Codes, scales and zeros of a weight matrix, one wave per group.  With zeros: the group's range with 0 in it over 15 steps; without: its largest
 // magnitude over 7 steps around code 8.  The scale is rounded to its type first, codes are the nearest (ties to even) under the rounded scale.
+// A group with a weight that is not finite has NaN for its scale, and its zero for codes.
 struct W4QuantArgs {
     const void* w; long ws;                       // [N][K], row stride in elements
     unsigned char* codes; long cs;
@@ -301,13 +302,16 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(W4QuantArgs a) {
     const int k0 = g * a.group, k1 = a.K - k0 < a.group ? a.K : k0 + a.group;
     const long wb = (long)n * a.ws;
     float lo = 0.f, hi = 0.f;
+    bool bad = false;
     for (int k = k0 + lane; k < k1; k += 64) {
         const float v = gd_load<T>(a.w, wb + k);
+        bad |= !gd_finite(v);
         lo = v < lo ? v : lo; hi = v > hi ? v : hi;
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o)); hi = fmaxf(hi, __shfl_xor(hi, o)); }
     float s = a.zeros ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f;
+    if (__any(bad)) s = gd_nan();                 // no code stands for it: the layer's output shows it
     if (lane == 0) gd_store<T>(a.scales, (long)n * a.ss + g, s);
     if constexpr (sizeof(T) == 2) {               // the value as it is stored
         if constexpr (__is_same(T, __half)) s = __half2float(__float2half(s));

@@ -256,7 +256,7 @@ def w4_quantize(weight: "torch.Tensor", *, group: int = 64, symmetric: bool = Fa
     """(codes, scales, zeros) of a weight matrix [N, K] for `w4_matvec`; scales have the weight's type, zeros is None where symmetric.
 
     A group's range, 0 included, is divided into 15 steps (symmetric: its largest magnitude into 7); codes are the nearest, ties to even, under
-    the scale as it is stored.  Rows of codes start at multiples of 16 bytes, which is what `w4_matvec` reads fastest."""
+    the scale as it is stored; a group with a weight that is not finite has the scale NaN.  Rows of codes start at multiples of 16 bytes, which is what `w4_matvec` reads fastest."""
     torch = _torch()
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be a torch tensor [N, K]")

@@ -262,7 +262,8 @@ typedef struct dpdf_w4_matvec_args {
 int dpdf_w4_matvec(int device, const dpdf_w4_matvec_args* args, void* stream);
 
 /* Codes, scales (and zeros, if not NULL) of a weight matrix [out_dim, in_dim].  With zeros a group's range, 0 included, is divided into 15
- * steps, without them its largest magnitude into 7; codes are the nearest (ties to even) under the scale as it is stored. */
+ * steps, without them its largest magnitude into 7; codes are the nearest (ties to even) under the scale as it is stored.  A group with a
+ * weight that is not finite gets the scale NaN, so that the layer's output shows it. */
 typedef struct dpdf_w4_quantize_args {
     int dtype;                               /* of weight and scales */
     int in_dim, out_dim, group;

@@ -942,6 +942,28 @@ def test_w4_quantize_is_the_formula(dtype, N, K, group):
         assert bool(((y - w.double().t()).abs() <= step * 0.5 * 1.1 + step * 8 * HALF_STEP[dtype] * 2).all())        # half a step, and the scale's own rounding over 8 to 15 steps
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_w4_quantize_shows_weights_that_are_not_finite(value, symmetric, dtype):
+    """The group's scale is NaN, its codes are the zero, every other group is what it was; the layer's outputs of that row are NaN."""
+    w = torch.randn(6, 200, generator=torch.Generator().manual_seed(3)).to(dtype).cuda()
+    codes, scales, zeros = operators.w4_quantize(w, symmetric=symmetric)
+    hit = torch.zeros_like(scales, dtype=torch.bool)
+    for n, k in ((1, 0), (2, 63), (3, 130), (5, 199)):
+        w[n, k] = value
+        hit[n, k // 64] = True
+    got, gs, gz = operators.w4_quantize(w, symmetric=symmetric)
+    assert bool(gs[hit].isnan().all()) and torch.equal(gs[~hit], scales[~hit])
+    cols = hit.repeat_interleave(32, 1)[:, :100]
+    assert torch.equal(got[~cols], codes[~cols]) and bool((got[cols] == (0x88 if symmetric else 0)).all())
+    if not symmetric:
+        assert torch.equal(gz[~hit], zeros[~hit]) and bool((gz[hit] == 0).all())
+    y = operators.w4_matvec(torch.ones(2, 200, dtype=dtype, device="cuda"), got, gs, zeros=gz)
+    assert torch.equal(y.isnan(), hit.any(1).expand(2, -1))
+
+
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # GPU: together, on streams, in graphs
 # ---------------------------------------------------------------------------------------------------------------------------------------
