@@ -310,7 +310,7 @@ __global__ __launch_bounds__(256) void w4_quantize_kernel(W4QuantArgs a) {
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o)); hi = fmaxf(hi, __shfl_xor(hi, o)); }
-    float s = a.zeros ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f;
+    float s = a.zeros ? (gd_finite(hi - lo) ? (hi - lo) / 15.f : hi / 15.f - lo / 15.f) : fmaxf(hi, -lo) / 7.f;      // a range may leave fp32, a step does not
     if (__any(bad)) s = gd_nan();                 // no code stands for it: the layer's output shows it
     if (lane == 0) gd_store<T>(a.scales, (long)n * a.ss + g, s);
     if constexpr (sizeof(T) == 2) {               // the value as it is stored

@@ -964,6 +964,19 @@ def test_w4_quantize_shows_weights_that_are_not_finite(value, symmetric, dtype):
     assert torch.equal(y.isnan(), hit.any(1).expand(2, -1))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_w4_quantize_of_a_range_that_fp32_does_not_hold(dtype):
+    """A group from -3e38 to 3e38: finite weights, a finite scale.  Its step is 4e37, half of it the most that a weight is off (and the scale's rounding over 8 steps)."""
+    w = torch.linspace(-3e38, 3e38, 64).to(dtype)[None]
+    codes, scales, zeros = operators.w4_quantize(w.cuda())
+    assert bool(scales.isfinite().all())
+    y, _ = w4_layer(torch.eye(64), codes, scales, zeros, None, 64)
+    step = float(scales.double())
+    assert abs(step / 4e37 - 1) < 0.01
+    assert float((y.t() - w.double()).abs().max()) <= step * (0.5 * 1.1 + 16 * HALF_STEP[dtype])
+
+
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # GPU: together, on streams, in graphs
 # ---------------------------------------------------------------------------------------------------------------------------------------
