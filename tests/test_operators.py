@@ -968,7 +968,7 @@ def test_w4_quantize_shows_weights_that_are_not_finite(value, symmetric, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_w4_quantize_of_a_range_that_fp32_does_not_hold(dtype):
     """A group from -3e38 to 3e38: finite weights, a finite scale.  Its step is 4e37, half of it the most that a weight is off (and the scale's rounding over 8 steps)."""
-    w = torch.linspace(-3e38, 3e38, 64).to(dtype)[None]
+    w = torch.linspace(-3e38, 3e38, 64, dtype=torch.float64).to(dtype)[None]        # in fp32 linspace itself overflows
     codes, scales, zeros = operators.w4_quantize(w.cuda())
     assert bool(scales.isfinite().all())
     y, _ = w4_layer(torch.eye(64), codes, scales, zeros, None, 64)
