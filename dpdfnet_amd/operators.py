@@ -4,8 +4,8 @@ hop, and dense layers with 4-bit weights for a few rows -- the parts of a recurr
 
 Tensors are torch tensors on one HIP device, float32, float16 or bfloat16; calls are queued on torch's current stream of that device,
 allocate nothing beside their results (and, for a few long clips, a workspace) through torch and wait for nothing, so they can be captured into a graph.  Sums, states and accumulators are fp32
-whatever the tensors' type.  There is no backward pass: tensors that require a gradient are refused while gradients are recorded.  Wrong
-types, shapes and overlaps raise ValueError, failures of the device RuntimeError."""
+whatever the tensors' type.  There is no derivative: tensors that require a gradient are refused while gradients are recorded, and tensors that
+carry a forward-mode tangent always.  Wrong types, shapes and overlaps raise ValueError, failures of the device RuntimeError."""
 from __future__ import annotations
 
 import ctypes
@@ -56,6 +56,8 @@ def _torch():
 class _Env:
     def __init__(self):
         torch = _torch()
+        from torch.autograd import forward_ad
+        self.forward_ad = forward_ad
         self.torch, self.tensor, self.grad, self.empty = torch, torch.Tensor, torch.is_grad_enabled, torch.empty
         self.dtypes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
         self.f32, self.u8, self.i32 = torch.float32, torch.uint8, torch.int32
@@ -121,6 +123,14 @@ def _gate_strides(env, device, index, shape, dtype, name: str, t):
     return _checked(device, (*shape, 1), dtype, name, t[..., None] if isinstance(t, env.tensor) and t.dim() == 3 else t).stride()
 
 
+def _no_tangents(env, **tensors) -> None:
+    """Outside a forward-mode level, the usual case, no tensor has a tangent and none is looked at."""
+    if getattr(env.forward_ad, "_current_level", 0) >= 0:
+        for name, t in tensors.items():
+            if isinstance(t, env.tensor) and env.forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} carries a tangent, and this operator has no derivative: take forward_ad.unpack_dual({name}).primal")
+
+
 def _packed(fields, *values) -> bytes:
     try:
         return fields.pack(*values)
@@ -136,6 +146,7 @@ def _call(env, fn, index, args, *workspace) -> None:
 
 def _gated(fn, q, k, v, g, beta, state_in, state_out, lengths, active, scale, out):
     env = _env()
+    _no_tangents(env, q=q, k=k, v=v, g=g, beta=beta, state=state_in, state_out=state_out, out=out)
     for name, t in (("q", q), ("v", v), ("g", g)):
         if not isinstance(t, env.tensor):
             raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -221,6 +232,7 @@ def w4_matvec(x: "torch.Tensor", codes: "torch.Tensor", scales: "torch.Tensor", 
     of x; zeros [N, ceil(K / group)] uint8, 0 .. 15 (8 everywhere if not given); bias [N] of the type of x; group a multiple of 32, the last
     one may be short.  `w4_quantize` makes codes, scales and zeros."""
     env = _env()
+    _no_tangents(env, x=x, scales=scales, bias=bias, out=out)
     for name, t in (("x", x), ("codes", codes), ("scales", scales)):
         if not isinstance(t, env.tensor):
             raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -260,6 +272,7 @@ def w4_quantize(weight: "torch.Tensor", *, group: int = 64, symmetric: bool = Fa
     torch = _torch()
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be a torch tensor [N, K]")
+    _no_tangents(_env(), weight=weight)
     code, group = _code(weight, "weight"), int(group)
     if group < 32 or group % 32:
         raise ValueError(f"group must be a multiple of 32, got {group}")

@@ -230,6 +230,18 @@ def test_python_layer_refuses_what_is_on_the_cpu_or_of_a_wrong_kind():
         operators.w4_quantize(torch.zeros(4, 64))
 
 
+def test_tangents_are_refused_before_anything_else():
+    from torch.autograd import forward_ad
+    q, k, v, g, beta = inputs(1, 2, 1, 2, 16, 16, F32, device="cpu")
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="v carries a tangent"):
+            operators.gated_delta(q, k, forward_ad.make_dual(v, v), g, beta)
+        with pytest.raises(ValueError, match="weight carries a tangent"):
+            operators.w4_quantize(forward_ad.make_dual(torch.zeros(4, 64), torch.ones(4, 64)))
+        with pytest.raises(ValueError, match="GPU"):
+            operators.gated_delta(q, k, v, g, beta)
+
+
 # ---------------------------------------------------------------------------------------------------------------------------------------
 # GPU: the gated delta rule
 # ---------------------------------------------------------------------------------------------------------------------------------------
@@ -730,6 +742,35 @@ def test_refusals_of_device_tensors():
     for change in (dict(codes=codes[:, :31]), dict(scales=scales.half()), dict(scales=scales[:, :0]), dict(zeros=scales), dict(bias=scales), dict(out=x), dict(codes=codes.int())):
         with pytest.raises(ValueError):
             operators.w4_matvec(**{**dict(x=x, codes=codes, scales=scales), **change})
+
+
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused():
+    """No derivative of either mode is computed, so that none is dropped silently."""
+    from torch.autograd import forward_ad
+    x = dict(zip("q k v g beta".split(), inputs(1, 3, 1, 2, 16, 16, F32)))
+    state = torch.zeros(1, 2, 16, 16, device="cuda")
+    y, codes, scales, _, bias = layer(2, 64, 8, 32, F32, False)
+    out = torch.zeros(1, 3, 2, 16, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for n, t in x.items():
+            with pytest.raises(ValueError, match="tangent"):
+                operators.gated_delta(**{**x, n: dual(t)})
+            with pytest.raises(ValueError, match="tangent"), torch.no_grad():
+                operators.gated_delta_step(**{**x, n: dual(t)}, state=state)
+        with pytest.raises(ValueError, match="tangent"):
+            operators.gated_delta(**x, state=dual(state))
+        with pytest.raises(ValueError, match="tangent"):
+            operators.gated_delta(**x, out=dual(out))
+        for change in (dict(x=dual(y)), dict(scales=dual(scales)), dict(bias=dual(bias))):
+            with pytest.raises(ValueError, match="tangent"):
+                operators.w4_matvec(**{**dict(x=y, codes=codes, scales=scales, bias=bias, group=32), **change})
+        with pytest.raises(ValueError, match="tangent"):
+            operators.w4_quantize(dual(y))
+        operators.gated_delta(**x)                                # a level alone changes nothing
+        operators.w4_matvec(y, codes, scales, group=32)
 
 
 @pytest.mark.gpu
