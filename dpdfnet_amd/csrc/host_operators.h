@@ -33,9 +33,12 @@ bool op_apart(const long* stride, const long* size, int dims, long last) {
     }
     return true;
 }
+constexpr long OP_THREADS = 0xffffffffL;          // of a launch, in one dimension
 int op_bytes(int dtype) { return dtype == DPDF_F32 ? 4 : dtype == DPDF_F16 || dtype == DPDF_BF16 ? 2 : 0; }
 bool op_aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
 
+int gd_columns(int Dk, int Dv, int dtype) { return Dv <= 32 && Dk <= 64 && dtype == DPDF_F32 ? 32 : Dv <= 64 ? 64 : 128; }
+int gd_columns(const GatedDeltaArgs& a, int dtype) { return gd_columns(a.Dk, a.Dv, dtype); }
 int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
     if (!p) return set_err(DPDF_E_INVALID, "null argument");
     const dpdf_gated_delta_args& x = *p;
@@ -49,8 +52,9 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
     if (step && x.lengths) return set_err(DPDF_E_INVALID, "gated delta rule: a step takes no lengths");
     if (!step && x.active) return set_err(DPDF_E_INVALID, "gated delta rule: clips take no mask of active streams");
     const long B = x.batch, T = x.frames, Hk = x.k_heads, Hv = x.v_heads, Dk = x.k_dim, Dv = x.v_dim;
-    const long states = (Dv + 31) / 32 * B * Hv;
-    if (states > 0x7fffffffL) return set_err(DPDF_E_INVALID, "gated delta rule: batch %d with %d heads of %d is too large for one call", x.batch, x.v_heads, x.v_dim);
+    // one wave to 32 columns of a hop, columns / 16 waves to as many of a clip; B Hv is below 2^62
+    const long columns = step ? 32 : gd_columns(x.k_dim, x.v_dim, x.dtype), threads = step ? 64 : 4 * columns;
+    if (B * Hv > OP_THREADS / threads || (Dv + columns - 1) / columns > OP_THREADS / threads / (B * Hv > 0 ? B * Hv : 1)) return set_err(DPDF_E_INVALID, "gated delta rule: batch %d with %d heads of %d is too large for one call", x.batch, x.v_heads, x.v_dim);
     if (B && (step && (!x.state_in || !x.state_out))) return set_err(DPDF_E_INVALID, "gated delta rule: a step needs its state");
     const long kd[3] = {B, T, Hk}, vd[3] = {B, T, Hv};
     for (const long* s : {x.q_stride, x.k_stride, x.v_stride, x.g_stride, x.beta_stride, x.out_stride})
@@ -98,11 +102,10 @@ void gd_pieces(GatedDeltaArgs& a, int e) {
     a.whole = a.Dk % 8 == 0 && gd_fours(a.q, a.qs, e) && gd_fours(a.k, a.ks, e);
     a.even = a.Dv % 4 == 0 && gd_fours(a.out, a.os, e);
 }
-// The frames of a chunk, the columns of a workgroup and the workgroups that a CU holds at once (registers and LDS).  Two waves for 32 columns
+// The frames of a chunk, the columns of a workgroup (gd_columns) and the workgroups that a CU holds at once (registers and LDS).  Two waves for 32 columns
 // where a chunk has two diagonal blocks for them: with four, half of them would have no column (104 clips x 2463 frames, 8 heads of 16, fp32:
 // 683 us with four, 366 with two; fp16 with its four blocks, 166 clips x 450 frames: 107 with four, 120 with two).
 int gd_chunk(int dtype) { return dtype == DPDF_F32 ? 32 : 64; }
-int gd_columns(const GatedDeltaArgs& a, int dtype) { return a.Dv <= 32 && a.Dk <= 64 && dtype == DPDF_F32 ? 32 : a.Dv <= 64 ? 64 : 128; }
 int gd_resident(const GatedDeltaArgs& a, int dtype) {
     const int columns = gd_columns(a, dtype);
     return columns == 128 || (a.Dk > 64 && dtype == DPDF_F16) ? 1 : columns == 64 ? 2 : a.Dk <= 32 ? 4 : 3;
@@ -161,10 +164,14 @@ int w4_tiles(const W4Args& a) {
     const long tiles = ((long)a.N + 15) / 16 * (((long)a.M + 15) / 16);
     return tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
 }
+// Four waves where a wave holds four tiles: two workgroups fit on a CU and start at once (8192 x 32768: 44 us, with eight waves 48)
+int w4_waves(const W4Args& a, int nt) {
+    const int units = (a.K + 127) / 128, most = nt == 4 ? W4_WAVES / 2 : W4_WAVES;
+    return units < most ? units : most;
+}
 template <typename T, typename G>
 void w4_launch(const W4Args& a, unsigned grid, int nt, hipStream_t s) {
-    // four waves where a wave holds four tiles: two workgroups fit on a CU and start at once (8192 x 32768: 44 us, with eight waves 48)
-    const int units = (a.K + 127) / 128, most = nt == 4 ? W4_WAVES / 2 : W4_WAVES, nw = units < most ? units : most;
+    const int nw = w4_waves(a, nt);
 #define W4_RUN_(R, N) w4_matvec_kernel<T, G, R, N><<<grid, 64 * nw, 0, s>>>(a)
 #define W4_RUN(R) (nt == 4 ? (W4_RUN_(R, 4)) : nt == 2 ? (W4_RUN_(R, 2)) : (W4_RUN_(R, 1)))
     if (a.group % 128 == 0) W4_RUN(4); else if (a.group % 64 == 0) W4_RUN(2); else W4_RUN(1);
@@ -296,7 +303,7 @@ extern "C" int dpdf_w4_matvec(int device, const dpdf_w4_matvec_args* args, void*
     const int nt = w4_tiles(a);
     a.tiles = (unsigned)((x.out_dim + 16L * nt - 1) / (16 * nt));
     const long grid = a.tiles * ((x.rows + 15L) / 16);
-    if (grid > 0x7fffffffL) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
+    if (grid > OP_THREADS / (64 * w4_waves(a, nt))) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
     OpDevice dev(device);
     HIP_TRY(dev.err);
     gd_types(x.dtype, x.scale_dtype, [&](auto t, auto g) { w4_launch<decltype(t), decltype(g)>(a, (unsigned)grid, nt, (hipStream_t)stream); });

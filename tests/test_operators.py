@@ -175,6 +175,23 @@ def test_lengths_and_masks_in_an_outputs_memory_are_refused(change):
     assert rc == -1 and "overlaps an input" in msg, (rc, msg)
 
 
+def test_calls_of_more_threads_than_a_launch_has_are_refused():
+    """2^32 threads: 2^26 heads of a step's one wave, 2^24 of a clip's four, tiles of up to eight waves; one less of them is no such case."""
+    far = {n: (i + 1) << 44 for i, n in enumerate(("q", "k", "v", "g", "beta", "out"))}
+    far.update({n + "_stride": (1, 1, 1) for n in far}, frames=1, k_heads=1, v_heads=1, k_dim=1, v_dim=1, state_in=8 << 44, state_out=8 << 44)
+    ok = 0 if backend.device_count() else -2
+    for step, most in ((True, 1 << 26), (False, 1 << 24)):
+        rc, msg = _c_gated(step=step, **{**far, "batch": most})
+        assert rc == -1 and "too large for one call" in msg, (rc, msg)
+        if ok:                                                                # where no device is there, what is not refused ends at that
+            assert _c_gated(step=step, **{**far, "batch": most - 1})[0] == ok
+    w4 = dict(in_dim=1024, x=1 << 44, x_stride=1024, codes=2 << 44, codes_pitch=512, scales=3 << 44, zeros=4 << 44, bias=5 << 44, out=6 << 44, out_dim=1 << 20, out_stride=1 << 20, scales_stride=32, zeros_pitch=32)
+    rc, msg = _c_w4(rows=1 << 14, **w4)                                       # 2^26 tiles, four to a workgroup of four waves
+    assert rc == -1 and "too many for one call" in msg, (rc, msg)
+    if ok:
+        assert _c_w4(rows=(1 << 14) - 16, **w4)[0] == ok
+
+
 def _c_w4(**change):
     v = dict(dtype=1, scale_dtype=1, rows=2, in_dim=100, out_dim=6, group=32, x=0x1000000, x_stride=100, codes=0x2000000, codes_pitch=50,
              scales=0x3000000, scales_stride=4, zeros=0x4000000, zeros_pitch=4, bias=0x5000000, out=0x6000000, out_stride=6)
