@@ -269,11 +269,11 @@ extern "C" int dpdf_w4_quantize(int device, const dpdf_w4_quantize_args* args, v
                      {(const char*)x.zeros, (const char*)x.zeros + (x.zeros ? (rows - 1) * x.zeros_pitch + groups : 0)}};
     for (int i = 0; i < 3; ++i)
         if (op_meet(w, o[i]) || op_meet(o[i], o[(i + 1) % 3])) return set_err(DPDF_E_INVALID, "w4 quantize: an output overlaps another tensor");
-    if ((long)x.out_dim * groups > 4 * 0x7fffffffL) return set_err(DPDF_E_INVALID, "w4 quantize: %d x %ld groups are too many for one call", x.out_dim, groups);
     OpDevice dev(device);
     HIP_TRY(dev.err);
     W4QuantArgs a{x.weight, x.weight_stride, x.codes, x.codes_pitch, x.scales, x.scales_stride, x.zeros, x.zeros_pitch, x.out_dim, x.in_dim, x.group, (int)groups};
-    const unsigned grid = (unsigned)(((long)x.out_dim * groups + 3) / 4);
+    const long need = ((long)x.out_dim * groups + 3) / 4, most = OP_THREADS / 256;      // four waves, a group each at a time
+    const unsigned grid = (unsigned)(need < most ? need : most);
     if (x.dtype == DPDF_F32) w4_quantize_kernel<float><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else if (x.dtype == DPDF_F16) w4_quantize_kernel<__half><<<grid, 256, 0, (hipStream_t)stream>>>(a);
     else w4_quantize_kernel<__hip_bfloat16><<<grid, 256, 0, (hipStream_t)stream>>>(a);

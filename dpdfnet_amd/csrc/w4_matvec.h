@@ -296,37 +296,37 @@ struct W4QuantArgs {
 template <typename T>
 __global__ __launch_bounds__(256) void w4_quantize_kernel(W4QuantArgs a) {
     const int lane = threadIdx.x & 63;
-    const long e = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (e >= (long)a.N * a.groups) return;
-    const int n = (int)(e / a.groups), g = (int)(e - (long)n * a.groups);
-    const int k0 = g * a.group, k1 = a.K - k0 < a.group ? a.K : k0 + a.group;
-    const long wb = (long)n * a.ws;
-    float lo = 0.f, hi = 0.f;
-    bool bad = false;
-    for (int k = k0 + lane; k < k1; k += 64) {
-        const float v = gd_load<T>(a.w, wb + k);
-        bad |= !gd_finite(v);
-        lo = v < lo ? v : lo; hi = v > hi ? v : hi;
-    }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o)); hi = fmaxf(hi, __shfl_xor(hi, o)); }
-    float s = a.zeros ? (gd_finite(hi - lo) ? (hi - lo) / 15.f : hi / 15.f - lo / 15.f) : fmaxf(hi, -lo) / 7.f;      // a range may leave fp32, a step does not
-    if (__any(bad)) s = gd_nan();                 // no code stands for it: the layer's output shows it
-    if (lane == 0) gd_store<T>(a.scales, (long)n * a.ss + g, s);
-    if constexpr (sizeof(T) == 2) {               // the value as it is stored
-        if constexpr (__is_same(T, __half)) s = __half2float(__float2half(s));
-        else s = (float)(__bf16)s;
-    }
-    const float z = a.zeros ? (s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f) : 8.f;
-    if (a.zeros && lane == 0) a.zeros[(long)n * a.zs + g] = (unsigned char)z;
-    for (int k = k0 + 2 * lane; k < k1; k += 128) {
-        unsigned c = 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float v = k + i < k1 ? gd_load<T>(a.w, wb + k + i) : 0.f;
-            const float r = s > 0.f ? rintf(v / s) + z : z;
-            c |= (unsigned)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+    for (long e = (long)blockIdx.x * 4 + (threadIdx.x >> 6); e < (long)a.N * a.groups; e += (long)gridDim.x * 4) {
+        const int n = (int)(e / a.groups), g = (int)(e - (long)n * a.groups);
+        const int k0 = g * a.group, k1 = a.K - k0 < a.group ? a.K : k0 + a.group;
+        const long wb = (long)n * a.ws;
+        float lo = 0.f, hi = 0.f;
+        bool bad = false;
+        for (int k = k0 + lane; k < k1; k += 64) {
+            const float v = gd_load<T>(a.w, wb + k);
+            bad |= !gd_finite(v);
+            lo = v < lo ? v : lo; hi = v > hi ? v : hi;
         }
-        a.codes[(long)n * a.cs + (k >> 1)] = (unsigned char)c;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { lo = fminf(lo, __shfl_xor(lo, o)); hi = fmaxf(hi, __shfl_xor(hi, o)); }
+        float s = a.zeros ? (gd_finite(hi - lo) ? (hi - lo) / 15.f : hi / 15.f - lo / 15.f) : fmaxf(hi, -lo) / 7.f;      // a range may leave fp32, a step does not
+        if (__any(bad)) s = gd_nan();                 // no code stands for it: the layer's output shows it
+        if (lane == 0) gd_store<T>(a.scales, (long)n * a.ss + g, s);
+        if constexpr (sizeof(T) == 2) {               // the value as it is stored
+            if constexpr (__is_same(T, __half)) s = __half2float(__float2half(s));
+            else s = (float)(__bf16)s;
+        }
+        const float z = a.zeros ? (s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f) : 8.f;
+        if (a.zeros && lane == 0) a.zeros[(long)n * a.zs + g] = (unsigned char)z;
+        for (int k = k0 + 2 * lane; k < k1; k += 128) {
+            unsigned c = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float v = k + i < k1 ? gd_load<T>(a.w, wb + k + i) : 0.f;
+                const float r = s > 0.f ? rintf(v / s) + z : z;
+                c |= (unsigned)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+            }
+            a.codes[(long)n * a.cs + (k >> 1)] = (unsigned char)c;
+        }
     }
 }

@@ -1001,6 +1001,18 @@ def test_w4_quantize_is_the_formula(dtype, N, K, group):
 
 
 @pytest.mark.gpu
+def test_w4_quantize_of_more_groups_than_a_launch_has_waves():
+    N, K = 2 ** 21 + 5, 1024
+    w = torch.empty(N, K, dtype=BF16, device="cuda")
+    w[:-9] = torch.randn(1, K, generator=torch.Generator().manual_seed(1)).cuda()
+    w[-9:] = torch.randn(9, K, generator=torch.Generator().manual_seed(2)).cuda()
+    codes, scales, zeros = operators.w4_quantize(w, group=32)
+    for rows in (slice(0, 3), slice(2 ** 20, 2 ** 20 + 3), slice(N - 9, N)):
+        c, s, z = operators.w4_quantize(w[rows].clone(), group=32)
+        assert torch.equal(codes[rows], c) and torch.equal(scales[rows], s) and torch.equal(zeros[rows], z)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("symmetric", [False, True])
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
