@@ -47,7 +47,8 @@ int gd_check(const dpdf_gated_delta_args* p, bool step, GatedDeltaArgs& a) {
     if (x.batch < 0 || x.frames < 0) return set_err(DPDF_E_INVALID, "gated delta rule: negative size batch=%d frames=%d", x.batch, x.frames);
     if (x.frames > 1 << 30) return set_err(DPDF_E_INVALID, "gated delta rule: %d frames are too large a number for one call", x.frames);
     if (x.k_heads < 1 || x.v_heads < 1 || x.v_heads % x.k_heads) return set_err(DPDF_E_INVALID, "gated delta rule: %d value heads are no multiple of %d key heads", x.v_heads, x.k_heads);
-    if (x.k_dim < 1 || x.k_dim > 128 || x.v_dim < 1) return set_err(DPDF_E_INVALID, "gated delta rule: head sizes %d (1 .. 128) and %d (from 1)", x.k_dim, x.v_dim);
+    // kernels count columns, inputs and outputs with 32 bits and go some hundred behind the last
+    if (x.k_dim < 1 || x.k_dim > 128 || x.v_dim < 1 || x.v_dim > 1 << 28) return set_err(DPDF_E_INVALID, "gated delta rule: head sizes %d (1 .. 128) and %d (1 .. 2^28)", x.k_dim, x.v_dim);
     if (!(x.scale - x.scale == 0.f)) return set_err(DPDF_E_INVALID, "gated delta rule: scale is not finite");
     if (step && x.lengths) return set_err(DPDF_E_INVALID, "gated delta rule: a step takes no lengths");
     if (!step && x.active) return set_err(DPDF_E_INVALID, "gated delta rule: clips take no mask of active streams");
@@ -182,6 +183,7 @@ void w4_launch(const W4Args& a, unsigned grid, int nt, hipStream_t s) {
 int w4_check(int dtype, long K, long N, int group, const char* what) {
     if (!op_bytes(dtype)) return set_err(DPDF_E_INVALID, "%s: unsupported dtype %d", what, dtype);
     if (K < 1 || N < 1) return set_err(DPDF_E_INVALID, "%s: empty layer %ld x %ld", what, N, K);
+    if (K > 1 << 30 || N > 1 << 30) return set_err(DPDF_E_INVALID, "%s: a layer of %ld x %ld is too large", what, N, K);
     if (group < 32 || group % 32) return set_err(DPDF_E_INVALID, "%s: group %d is no multiple of 32", what, group);
     return DPDF_OK;
 }

@@ -214,7 +214,7 @@ enum { DPDF_F32 = 0, DPDF_F16 = 1, DPDF_BF16 = 2 };
 /* The gated delta rule, a recurrence over frames with a matrix state S [k_dim][v_dim] per sequence and value head:
  *   S' = exp(g_t) S_{t-1};  e_t = beta_t (v_t - S'^T k_t);  S_t = S' + k_t e_t^T;  out_t = scale S_t^T q_t
  * q, k [batch, frames, k_heads, k_dim]; v, out [batch, frames, v_heads, v_dim]; g, beta [batch, frames, v_heads];
- * state_in, state_out [batch, v_heads, k_dim, v_dim] fp32, contiguous.  Clips: 64 frames of a tensor span less than 2 GiB.  k_dim 1 .. 128;
+ * state_in, state_out [batch, v_heads, k_dim, v_dim] fp32, contiguous.  Clips: 64 frames of a tensor span less than 2 GiB.  k_dim 1 .. 128, v_dim to 2^28;
  * v_heads a multiple of k_heads, value head h reads key head h / (v_heads / k_heads).  The state is held, and every sum taken, in fp32.
  * g = -inf resets the state. */
 typedef struct dpdf_gated_delta_args {
@@ -246,7 +246,7 @@ int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* args, void* s
 
 /* Dense layers with 4-bit weights: out[m][n] = sum_k x[m][k] (code[n][k] - zero[n][k / group]) scale[n][k / group] + bias[n], sums in fp32.
  * Codes are two to a byte, the lower half first (codes [out_dim, (in_dim + 1) / 2]); scales, zeros [out_dim, ceil(in_dim / group)];
- * group a multiple of 32, the last one may be short.  Products x (code - zero) are exact; a group's sum of them, in fp32, is taken before its scale and
+ * group a multiple of 32, the last one may be short; in_dim and out_dim to 2^30.  Products x (code - zero) are exact; a group's sum of them, in fp32, is taken before its scale and
  * has to stay in fp32's range.  A value of x that is not finite makes its row's outputs so (NaN where the formula has an infinity), a scale its
  * output's. */
 typedef struct dpdf_w4_matvec_args {

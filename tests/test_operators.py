@@ -175,6 +175,20 @@ def test_lengths_and_masks_in_an_outputs_memory_are_refused(change):
     assert rc == -1 and "overlaps an input" in msg, (rc, msg)
 
 
+def test_sizes_next_to_what_32_bits_count_are_refused():
+    big = (1 << 30) + 1
+    for change in (dict(in_dim=big), dict(out_dim=big), dict(in_dim=(1 << 31) - 1), dict(out_dim=(1 << 31) - 1, out_stride=(1 << 31) - 1)):
+        change = dict(x=1 << 44, x_stride=1 << 32, codes=2 << 44, codes_pitch=1 << 31, scales=3 << 44, scales_stride=1 << 27, zeros=4 << 44, zeros_pitch=1 << 27, bias=5 << 44,
+                      out=6 << 44, out_stride=big) | change
+        rc, msg = _c_w4(**change)
+        assert rc == -1 and "too large" in msg, (rc, msg)
+    a = operators._W4QuantizeArgs(0, (1 << 31) - 1, 1, 32, 1 << 44, 1 << 31, 2 << 44, 1 << 31, 3 << 44, 1 << 27, None, 0)
+    L = backend.load_library()
+    assert L.dpdf_w4_quantize(0, ctypes.addressof(a), None) == -1 and "too large" in L.dpdf_last_error().decode()
+    rc, msg = _c_gated(frames=0, batch=1, k_heads=1, v_heads=1, k_dim=1, v_dim=(1 << 31) - 1, state_in=1 << 44, state_out=2 << 44)
+    assert rc == -1 and "head sizes" in msg, (rc, msg)
+
+
 def test_calls_of_more_threads_than_a_launch_has_are_refused():
     """2^32 threads: 2^26 heads of a step's one wave, 2^24 of a clip's four, tiles of up to eight waves; one less of them is no such case."""
     far = {n: (i + 1) << 44 for i, n in enumerate(("q", "k", "v", "g", "beta", "out"))}
