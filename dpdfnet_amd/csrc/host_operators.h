@@ -159,20 +159,30 @@ template <typename F> void gd_types(int dtype, int gate, F f) {
     else { if (gate == DPDF_F32) f(__hip_bfloat16(), float()); else f(__hip_bfloat16(), __hip_bfloat16()); }
 }
 
-// Tiles of 16 outputs to a workgroup: few where the chip would not be full, many so that x is read less often.  Measured with 1, 2, 4:
-// 4096 x 4096, 16 rows (256 tiles) 8.1, 9.9, 13.8 us; 4096 x 16384, 1 row (1024) 13.7, 11.7, 12.1; 8192 x 32768, 8 rows (2048) 62, 50, 44.
-int w4_tiles(const W4Args& a) {
-    const long tiles = ((long)a.N + 15) / 16 * (((long)a.M + 15) / 16);
-    return tiles >= 2048 ? 4 : tiles >= 1024 ? 2 : 1;
-}
-// Four waves where a wave holds four tiles: two workgroups fit on a CU and start at once (8192 x 32768: 44 us, with eight waves 48)
-int w4_waves(const W4Args& a, int nt) {
-    const int units = (a.K + 127) / 128, most = nt == 4 ? W4_WAVES / 2 : W4_WAVES;
-    return units < most ? units : most;
+// Tiles of 16 outputs to a workgroup (nt) and its waves (nw), by the tiles that there are for each CU: few where the chip would not be full, many
+// so that x is read less often.  us with nt of 1, 2, 4, weights from HBM, K = 4096 and 128 to a group where nothing else is said:
+//     up to one for each CU    1.0: 8 rows of bf16 6.5, 8.2, 12.3; 2 of fp32 8.6, 10.7, 16.8; 8 of fp16, group 32 7.2, 10.3, 16.1
+//     up to two                1.2: 1 of bf16, K = 8192 13.8, 12.8, 20.4; 1.8: 4 of fp16, group 64 10.5, 9.2, 14.2; 2.0: 2 of fp32 13.8, 12.0, 18.2
+//     more                     3.5: 8 of bf16 18.2, 14.6, 14.0; 6: 2 of fp32 35.5, 31.8, 29.0; 8: 16 of bf16, K = 1024, group 64 26.7, 22.4, 10.7
+// The last round of workgroups counts whole: with long sums of 16-bit rows, which are bound by reading codes, two are better where four would leave
+// more of it empty (5: 8 of bf16 22.2, 19.6, 22.8; 10: 1 of bf16, K = 8192 56.6, 48.2, 53.5; but 1 of bf16, K = 1024 18.4, 14.2, 10.8; 16: 8 of bf16 62.4, 47.1, 43.5),
+// and for one row or two, whose x costs little, up to eight (4: 15.1, 12.5, 14.1; 8: 27.3, 22.3, 23.3; with 4 rows, K = 8192, 3: 23.1, 23.2, 22.0).
+// With four tiles, four waves, of which two workgroups fit on a CU and start at once (6: 2 of fp32 29.0 us, with eight waves 32.0), but eight where fp32
+// rows have one workgroup to a CU at most (3.5: 18.7, with eight 17.1; 8 of bf16 14.0 and 14.3).
+struct W4Split { int nt, nw; };
+W4Split w4_split(const W4Args& a, int dtype, int cus) {
+    const long tiles = ((long)a.N + 15) / 16 * (((long)a.M + 15) / 16), units = ((long)a.K + 127) / 128;
+    int nt = tiles <= cus ? 1 : tiles <= 2L * cus ? 2 : 4, nw = W4_WAVES;
+    if (nt == 4 && dtype != DPDF_F32 && a.group % 128 == 0 && a.K >= 4096 && tiles <= 10L * cus) {
+        const long two = (tiles + 2 * cus - 1) / (2 * cus) * 2, four = (tiles + 4 * cus - 1) / (4 * cus) * 4;
+        if (two < four || (a.M <= 2 && tiles <= 8L * cus)) nt = 2;
+    }
+    if (nt == 4 && (dtype != DPDF_F32 || tiles > 4L * cus)) nw = W4_WAVES / 2;
+    return {nt, (int)(units < nw ? units : nw)};
 }
 template <typename T, typename G>
-void w4_launch(const W4Args& a, unsigned grid, int nt, hipStream_t s) {
-    const int nw = w4_waves(a, nt);
+void w4_launch(const W4Args& a, unsigned grid, W4Split split, hipStream_t s) {
+    const int nt = split.nt, nw = split.nw;
 #define W4_RUN_(R, N) w4_matvec_kernel<T, G, R, N><<<grid, 64 * nw, 0, s>>>(a)
 #define W4_RUN(R) (nt == 4 ? (W4_RUN_(R, 4)) : nt == 2 ? (W4_RUN_(R, 2)) : (W4_RUN_(R, 1)))
     if (a.group % 128 == 0) W4_RUN(4); else if (a.group % 64 == 0) W4_RUN(2); else W4_RUN(1);
@@ -302,13 +312,16 @@ extern "C" int dpdf_w4_matvec(int device, const dpdf_w4_matvec_args* args, void*
                           {(const char*)x.zeros, (const char*)x.zeros + (x.zeros ? (x.out_dim - 1L) * x.zeros_pitch + groups : 0)}, {(const char*)x.bias, (const char*)x.bias + (x.bias ? (long)x.out_dim * e : 0)}};
     for (const OpSpan& i : in) if (op_meet(o, i)) return set_err(DPDF_E_INVALID, "w4 matvec: out overlaps an input");
     W4Args a{x.x, x.x_stride, x.codes, x.codes_pitch, x.scales, x.scales_stride, x.zeros, x.zeros_pitch, x.bias, x.out, x.out_stride, x.rows, x.in_dim, x.out_dim, x.group, 0};
-    const int nt = w4_tiles(a);
+    int cus = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess) cus = 256;      // a missing device is reported below
+    const W4Split split = w4_split(a, x.dtype, cus);
+    const int nt = split.nt;
     a.tiles = (unsigned)((x.out_dim + 16L * nt - 1) / (16 * nt));
     const long grid = a.tiles * ((x.rows + 15L) / 16);
-    if (grid > OP_THREADS / (64 * w4_waves(a, nt))) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
+    if (grid > OP_THREADS / (64 * split.nw)) return set_err(DPDF_E_INVALID, "w4 matvec: %d rows are too many for one call", x.rows);
     OpDevice dev(device);
     HIP_TRY(dev.err);
-    gd_types(x.dtype, x.scale_dtype, [&](auto t, auto g) { w4_launch<decltype(t), decltype(g)>(a, (unsigned)grid, nt, (hipStream_t)stream); });
+    gd_types(x.dtype, x.scale_dtype, [&](auto t, auto g) { w4_launch<decltype(t), decltype(g)>(a, (unsigned)grid, split, (hipStream_t)stream); });
     HIP_TRY(hipGetLastError());
     return DPDF_OK;
 }

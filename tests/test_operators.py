@@ -927,6 +927,21 @@ def test_w4_rows_are_independent_and_repeat(dtype, M):
     assert torch.equal(got[:, keep], y[:, keep]) and not bool(torch.isfinite(got[:, 5]).any())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("scales32", [True, False])
+@pytest.mark.parametrize("M, K, N, group", [(3, 1300, 5000, 32), (3, 1300, 5000, 64), (3, 1300, 5000, 128), (20, 700, 4000, 96), (2, 4100, 20000, 128), (9, 4096, 20480, 128),
+                                            (9, 4100, 14000, 128), (9, 1300, 14000, 64), (1, 300, 70000, 32)])
+def test_w4_layers_between_the_splits(M, K, N, group, scales32, dtype):
+    """One, two and four tiles to a workgroup and four and eight waves, by tiles for each CU: 1.2, 1.9, 2 - 5, 17."""
+    x, codes, scales, z, bias = layer(M, K, N, group, dtype, group == 64, seed=N, scale_dtype=F32 if scales32 else None)
+    y = operators.w4_matvec(x, codes, scales, zeros=z, bias=bias, group=group)
+    at = torch.cat([torch.arange(0, N, 997), torch.arange(N - 40, N)]).cuda()
+    ref, mag = w4_layer(x, codes[at], scales[at], None if z is None else z[at], bias[at], group)
+    near_layer(y[:, at], ref, mag, K, dtype)
+    assert torch.equal(y, operators.w4_matvec(x, codes, scales, zeros=z, bias=bias, group=group))
+
+
 def near_sparse_layer(y, x, codes, scales, z, group, dtype):
     """Weights near their zero: a term whose code is the zero is 0 and adds nothing, the n others of an output are at most three products each (fp32 rows
     are three limbs) with one sum each, and a scale and a sum per group: 8 deviations of sqrt(5 n) roundings of the terms' magnitudes."""
