@@ -20,7 +20,8 @@ struct W4Args {
 // time is that of reading the codes), the weights are the right one, as code - zero, which both 16-bit types hold exactly: a term whose code is
 // the zero is 0, products are exact, and the sums' roundings go by the terms alone.  A group's sum is taken before its scale.
 // Four codes to a word of bytes, e = 128 + zero - code: from 128 on that is a sign and |code - zero|, below it 128 - e is, and a byte of a
-// sign and 0 .. 15 is that many steps of 2^-9 as an 8-bit float (e4m3, whose steps are even up to there): 17 instructions for eight weights.
+// sign and 0 .. 15 is that many steps of 2^-9 as an 8-bit float (e4m3, whose steps are even up to there): 17 instructions for eight weights.  A zero
+// above 15 has no such bytes; its group's scale counts as NaN.
 // Codes 0 2 4 6 and 1 3 5 7 of a word come out together, so x is brought into that order.  fp32 rows go in as three bf16 limbs
 // (exact, see gru_limb.h), three products each.
 //
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(64 * W4_WAVES) void w4_matvec_kernel(W4Args a) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int u = 0; u < SUB; ++u) sc[SUB * q + u][16 * t + n] = make_float2(gd_load<G>(&s[t][u], 0), __builtin_bit_cast(float, zeros ? 0x01010101u * (128u + z[t][u]) : 0x88888888u));
+            for (int u = 0; u < SUB; ++u) sc[SUB * q + u][16 * t + n] = make_float2(zeros && z[t][u] > 15 ? gd_nan() : gd_load<G>(&s[t][u], 0), __builtin_bit_cast(float, zeros ? 0x01010101u * (128u + z[t][u]) : 0x88888888u));
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
     // one block, the j-th of the four whose scales are in LDS

@@ -248,7 +248,7 @@ int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* args, void* s
  * Codes are two to a byte, the lower half first (codes [out_dim, (in_dim + 1) / 2]); scales, zeros [out_dim, ceil(in_dim / group)];
  * group a multiple of 32, the last one may be short; in_dim and out_dim to 2^30.  Products x (code - zero) are exact; a group's sum of them, in fp32, is taken before its scale and
  * has to stay in fp32's range.  A value of x that is not finite makes its row's outputs so (NaN where the formula has an infinity), a scale its
- * output's. */
+ * output's; a zero above 15 makes its output NaN. */
 typedef struct dpdf_w4_matvec_args {
     int dtype, scale_dtype;                  /* of x, bias, out; of scales: DPDF_F32 or dtype */
     int rows, in_dim, out_dim, group;

@@ -981,6 +981,20 @@ def test_w4_weights_near_their_zero(M, K, N, group, zero, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_w4_zeros_above_15_show(group, dtype):
+    x, codes, scales, z, _ = layer(2, 610, 60, group, dtype, True, seed=group)
+    y = operators.w4_matvec(x, codes, scales, zeros=z, group=group)
+    hit = torch.zeros(60, dtype=torch.bool, device="cuda")
+    for n, at, v in ((3, 0, 16), (20, 1, 255), (40, scales.shape[1] - 1, 128), (59, 2, 31)):
+        z[n, at] = v
+        hit[n] = True
+    got = operators.w4_matvec(x, codes, scales, zeros=z, group=group)
+    assert torch.equal(got[:, ~hit], y[:, ~hit]) and bool(got[:, hit].isnan().all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_w4_large_inputs_are_not_taken_out_of_range(dtype):
     """|x| of 2e37, two in a row: their products with code - zero, 8 at most, stay below 3.4e38, and so does their sum."""
