@@ -233,7 +233,8 @@ typedef struct dpdf_gated_delta_args {
 /* Whole clips, in chunks of 32 or 64 frames.  Frames behind a clip's length are neither read nor written; state_out is the state after its last
  * frame (a clip of length 0: the state it came with).  A non-finite k, g (but -inf) or beta makes the outputs of its head from its frame
  * on, and its state, NaN, a non-finite v those of its column, a non-finite q those of its frame; nothing earlier and no other head.  Where positive g
- * add up to more than 88 inside a chunk (exp of it leaves fp32), the frame where they do counts as one of a non-finite g.
+ * add up to more than 88 inside a chunk (exp of it leaves fp32), the frame where they do counts as one of a non-finite g.  Sums of finite
+ * values that leave fp32's range by themselves may make earlier frames of their chunk NaN as well.
  *
  * Few heads over many frames are cut into segments that run side by side, given a workspace for the segments' states:
  * dpdf_gated_delta_workspace() bytes on the device, aligned to 16, the call's alone until it has run; 0 where there is nothing to cut.
@@ -241,7 +242,7 @@ typedef struct dpdf_gated_delta_args {
 size_t dpdf_gated_delta_workspace(int device, const dpdf_gated_delta_args* args);
 int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, void* workspace, size_t workspace_bytes, void* stream);
 /* `frames` hops (one, or a few) of every active stream, frame by frame; state_in is required, state_out = state_in updates it in place.
- * Rows of streams that are left out are neither read nor written.  k_dim x v_dim at most 2^28. */
+ * Rows of streams that are left out are neither read nor written; with 0 frames nothing is.  k_dim x v_dim at most 2^28. */
 int dpdf_gated_delta_step(int device, const dpdf_gated_delta_args* args, void* stream);
 
 /* Dense layers with 4-bit weights: out[m][n] = sum_k x[m][k] (code[n][k] - zero[n][k / group]) scale[n][k / group] + bias[n], sums in fp32.

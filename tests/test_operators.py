@@ -666,6 +666,31 @@ def test_few_long_clips_are_cut_into_segments(T, lens, Hk, Hv, Dk, Dv, dtype):
 
 
 @pytest.mark.gpu
+def test_captured_segments_update_a_state_in_place():
+    """Replays go on from where the last one ended; the captured call's workspace is the graph's own."""
+    x = inputs(2, 1200, 1, 2, 64, 64, BF16, seed=3, g_std=3.0)
+    lengths = torch.tensor((1200, 100), dtype=torch.int32, device="cuda")
+    state = torch.zeros(2, 2, 64, 64, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        operators.gated_delta(*x, state=state.clone(), lengths=lengths)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g in graphs:                                              # two of them, on the same state
+        with torch.cuda.graph(g):
+            outs.append(operators.gated_delta(*x, state=state, lengths=lengths, state_out=state)[0])
+    mirror = 0.5 * torch.randn(2, 2, 64, 64, generator=torch.Generator().manual_seed(1)).cuda()
+    state.copy_(mirror)
+    for r in range(4):
+        x[2].copy_(torch.randn(2, 1200, 2, 64, generator=torch.Generator().manual_seed(r)))
+        graphs[r % 2].replay()
+        want, mirror = operators.gated_delta(*x, state=mirror, lengths=lengths)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[r % 2], want) and torch.equal(state, mirror)
+
+
+@pytest.mark.gpu
 def test_a_workspace_over_the_lengths_is_refused():
     B, T, H, D = 1, 1200, 1, 64
     x = inputs(B, T, H, H, D, D, F32)
