@@ -123,12 +123,15 @@ def _gate_strides(env, device, index, shape, dtype, name: str, t):
     return _checked(device, (*shape, 1), dtype, name, t[..., None] if isinstance(t, env.tensor) and t.dim() == 3 else t).stride()
 
 
-def _no_tangents(env, **tensors) -> None:
+def _forward_mode(env) -> bool:
     """Outside a forward-mode level, the usual case, no tensor has a tangent and none is looked at."""
-    if getattr(env.forward_ad, "_current_level", 0) >= 0:
-        for name, t in tensors.items():
-            if isinstance(t, env.tensor) and env.forward_ad.unpack_dual(t).tangent is not None:
-                raise ValueError(f"{name} carries a tangent, and this operator has no derivative: take forward_ad.unpack_dual({name}).primal")
+    return getattr(env.forward_ad, "_current_level", 0) >= 0
+
+
+def _no_tangents(env, **tensors) -> None:
+    for name, t in tensors.items():
+        if isinstance(t, env.tensor) and env.forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{name} carries a tangent, and this operator has no derivative: take forward_ad.unpack_dual({name}).primal")
 
 
 def _packed(fields, *values) -> bytes:
@@ -146,7 +149,8 @@ def _call(env, fn, index, args, *workspace) -> None:
 
 def _gated(fn, q, k, v, g, beta, state_in, state_out, lengths, active, scale, out):
     env = _env()
-    _no_tangents(env, q=q, k=k, v=v, g=g, beta=beta, state=state_in, state_out=state_out, out=out)
+    if _forward_mode(env):
+        _no_tangents(env, q=q, k=k, v=v, g=g, beta=beta, state=state_in, state_out=state_out, out=out)
     for name, t in (("q", q), ("v", v), ("g", g)):
         if not isinstance(t, env.tensor):
             raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -232,7 +236,8 @@ def w4_matvec(x: "torch.Tensor", codes: "torch.Tensor", scales: "torch.Tensor", 
     of x; zeros [N, ceil(K / group)] uint8, 0 .. 15 (8 everywhere if not given); bias [N] of the type of x; group a multiple of 32, the last
     one may be short.  `w4_quantize` makes codes, scales and zeros."""
     env = _env()
-    _no_tangents(env, x=x, scales=scales, bias=bias, out=out)
+    if _forward_mode(env):
+        _no_tangents(env, x=x, scales=scales, bias=bias, out=out)
     for name, t in (("x", x), ("codes", codes), ("scales", scales)):
         if not isinstance(t, env.tensor):
             raise ValueError(f"{name} must be a torch tensor, got {type(t).__name__}")
@@ -272,7 +277,8 @@ def w4_quantize(weight: "torch.Tensor", *, group: int = 64, symmetric: bool = Fa
     torch = _torch()
     if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
         raise ValueError("weight must be a torch tensor [N, K]")
-    _no_tangents(_env(), weight=weight)
+    if _forward_mode(_env()):
+        _no_tangents(_env(), weight=weight)
     code, group = _code(weight, "weight"), int(group)
     if group < 32 or group % 32:
         raise ValueError(f"group must be a multiple of 32, got {group}")
