@@ -222,9 +222,9 @@ __global__ __launch_bounds__(64) void gated_delta_step_kernel(GatedDeltaArgs a) 
 //
 // Bound: neither bytes nor products but the chain through a chunk, about 14 thousand cycles of which two workgroups on a CU overlap: K and Q into LDS
 // 1.4 thousand, the next chunk's loads 1 to 1.8, the blocks of A and P 1.8, inverses and the other blocks 2, K S and Q S 2, u, the outputs
-// and S 5 (4 heads of 64, bf16; vector units 42 % busy, matrix units 27 %; outputs then had two limbs, 174 us).  256 clips of 334 to 1003
-// frames, 4 heads of 64, bf16: 193 us, 1.9 TB/s; one recording of 16384 frames, 16 heads of 128: 413 us, in 16 segments.  With outputs of two
-// limbs these took 174 and 396 us (2.2 ms in one segment), and chunks of 32 frames in 16-bit types 228 and 532.
+// and S 5 (4 heads of 64, bf16; vector units 42 % busy, matrix units 27 %; counted with outputs of two limbs, 6 % faster).  The first four do not
+// depend on S and could be made ahead of it.  256 clips of 334 to 1003 frames, 4 heads of 64, bf16: 176 us, 2.1 TB/s; one recording of 16384 frames,
+// 16 heads of 128: 407 us, in 16 segments (2.26 ms in one).  Chunks of 32 frames in 16-bit types took a third longer.
 //
 // gamma and its differences are 64-bit: they are small differences of long sums.  A non-finite k, g or beta makes its head's outputs from its
 // frame on, and the final state, NaN; a non-finite v does that to its column; earlier frames stay as they are (the products run over all

@@ -104,8 +104,8 @@ void gd_pieces(GatedDeltaArgs& a, int e) {
     a.even = a.Dv % 4 == 0 && gd_fours(a.out, a.os, e);
 }
 // The frames of a chunk, the columns of a workgroup (gd_columns) and the workgroups that a CU holds at once (registers and LDS).  Two waves for 32 columns
-// where a chunk has two diagonal blocks for them: with four, half of them would have no column (104 clips x 2463 frames, 8 heads of 16, fp32:
-// 683 us with four, 366 with two; fp16 with its four blocks, 166 clips x 450 frames: 107 with four, 120 with two).
+// where a chunk has two diagonal blocks for them: with four, half of them would have no column (104 clips of 821 to 2463 frames, 8 heads of 16, fp32:
+// 427 us with four, 343 with two; 30 of 700 frames, 8 heads of 48 x 32: 112 and 103; fp16 with its four blocks, 166 clips x 450 frames: 107 with four, 120 with two).
 int gd_chunk(int dtype) { return dtype == DPDF_F32 ? 32 : 64; }
 int gd_resident(const GatedDeltaArgs& a, int dtype) {
     const int columns = gd_columns(a, dtype);
@@ -113,8 +113,9 @@ int gd_resident(const GatedDeltaArgs& a, int dtype) {
 }
 // Segments for `heads` heads: as many as fill the chip once, and only where the chip would hold three times the workgroups there are.  A segment costs
 // its frames about one and a half times more and a step of the join, a seventh of a chunk: hence no more than the root of five times the
-// chunks (6 heads, 48 chunks: 49 us in 12 segments, 45 in 16, 53 in 24), and at least two chunks each, four where the second pass would start in
-// several rounds (2 clips of 17 chunks, 4 heads: 36 us by two, 52 by four; 111 heads, 14 chunks: 150 and 106).
+// chunks (6 heads, 50 chunks: 67 us in 10 segments, 60 in 13, 56 in 17, 60 in 25; 3 heads, 100 chunks: 81 in 17, 76 in 20, 83 in 50), and at least two
+// chunks each, four where the second pass would start in several rounds (2 clips of 17 chunks, 4 heads: 43 us by three, 59 by five;
+// 111 heads, 14 chunks: 94 by two, 75 by five, 80 in one piece).
 int gd_segments(const GatedDeltaArgs& a, int dtype, long heads, int cus) {
     const long strips = (a.Dv + gd_columns(a, dtype) - 1) / gd_columns(a, dtype), groups = heads * strips, room = (long)cus * gd_resident(a, dtype);
     const long chunks = ((long)a.T + gd_chunk(dtype) - 1) / gd_chunk(dtype);
@@ -241,7 +242,7 @@ extern "C" int dpdf_gated_delta(int device, const dpdf_gated_delta_args* args, v
     if (a.lengths && a.segments == 1 && a.B <= 4 * gd_columns(a, args->dtype) && a.B <= GD_RANKED && a.T < 1 << 25) {
         int cus = 0;
         HIP_TRY(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, device));
-        // all of them start at once otherwise (256 clips of 334 to 1003 frames, 4 heads of 64 in bf16: 205 us in the batch's order, 178 us so)
+        // all of them start at once otherwise (256 clips of 334 to 1003 frames, 4 heads of 64 in bf16: 210 us in the batch's order, 175 us so); of more clips than threads, the batch's order stays
         a.sorted = heads * ((a.Dv + gd_columns(a, args->dtype) - 1) / gd_columns(a, args->dtype)) > (long)cus * gd_resident(a, args->dtype);
     }
     gd_type(args->dtype, [&](auto t) { gd_launch_clips<decltype(t)>(a, heads, (hipStream_t)stream); });

@@ -33,8 +33,8 @@ struct W4Args {
 //
 // Bound: reading the codes; what keeps it from a plain read's rate (24.6 us for the codes of 8192 x 32768, 5.5 TB/s) is the traffic beside them,
 // x about 7 us and scales 5, and the instructions for code - zero (16 + code, with (16 + zero) sum x taken off a group's sum, took 8 for eight weights and
-// 44 us, but its error went by 16 to 31 times |x|).  8192 x 32768, eight rows of bf16: 47 us, 3.0 TB/s; 4096 x 16384, one row: 12.3 us, 2.8 TB/s; 4096 x 4096, 16 rows:
-// 8.0 us.
+// 5 % less time, but its error went by 16 to 31 times |x|).  8192 x 32768, eight rows of bf16: 42.6 us, 3.3 TB/s; 4096 x 16384, one row: 11.5 us, 3.0 TB/s;
+// 4096 x 4096, 16 rows of fp16: 8.0 us.
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 template <typename T> struct W4X;                 // eight inputs of a row as a left operand: LIMBS fragments
